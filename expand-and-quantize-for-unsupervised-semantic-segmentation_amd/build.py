@@ -16,11 +16,13 @@ LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 OBJ_DIR = os.path.join(PKG_DIR, "build")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value",
-         "-ffp-contract=on"]
-# Per-file additions.  -fno-slp-vectorize for the attention kernel: its softmax sits between MFMAs,
-# where the packed fp32 ops (v_pk_add_f32 / v_pk_mul_f32) the SLP vectoriser forms issue slower than
-# the scalar pairs they replace (measured: 315 -> 288 us per launch).  The GEMM epilogues are faster
-# with it left on.
+         "-ffp-contract=on",
+         # No packed fp32 arithmetic (v_pk_add_f32 / v_pk_mul_f32 / v_pk_fma_f32): some of its forms have given wrong
+         # results on this part now and then.  Every lane computes the same IEEE operations without it; the 64 x 320x320
+         # eval step takes the same time (8.94 ms with and without).  (The host pass warns that it does not know the feature.)
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+# Per-file additions.  -fno-slp-vectorize for the attention kernel: its softmax sits between MFMAs, where the pairs the
+# SLP vectoriser forms issued slower than the scalar operations they replace.
 FILE_FLAGS = {"attention.hip": ["-fno-slp-vectorize"]}
 
 
@@ -61,7 +63,7 @@ def build_library(force=False, verbose=True, jobs=None):
     for src in _sources():
         obj = os.path.join(OBJ_DIR, src[:-4] + ".o")
         objs.append(obj)
-        if force or _stale(obj, [os.path.join(CSRC, src)] + hdrs):
+        if force or _stale(obj, [os.path.join(CSRC, src), os.path.abspath(__file__)] + hdrs):
             todo.append((os.path.join(CSRC, src), obj))
 
     def compile_one(item):

@@ -68,8 +68,8 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 // evaluation included), far below the bf16 rounding of the stored result; 5 fma + v_exp + max + fma
 // instead of the rcp + exp + 14 ops of Abramowitz-Stegun 7.1.26 or the ~30 branchy ops of erff.
 // Q's leading coefficient is negative, so large |x| gives 2^Q = 0 without a clamp (x = +-inf gives NaN).
-// Two values at a time: the packed fp32 fma issues once for both (|x| = 2 max(x, 0) - x is exact and
-// saves the two sign-bit masks; there is no packed max or exp).
+// Two values at a time, so that the two chains interleave (|x| = 2 max(x, 0) - x is exact and saves the
+// two sign-bit masks).
 typedef float gelu_f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ gelu_f32x2 gelu_erf2(gelu_f32x2 x) {
     const gelu_f32x2 relu = {fmaxf(x.x, 0.f), fmaxf(x.y, 0.f)};
@@ -85,7 +85,7 @@ __device__ __forceinline__ gelu_f32x2 gelu_erf2(gelu_f32x2 x) {
 }
 
 // The same for four pairs at a time with the steps of the four evaluations interleaved (same operations per element, so
-// the same bits): a lone evaluation is a chain of dependent packed fmas, each waiting for the one before.
+// the same bits): a lone evaluation is a chain of dependent fmas, each waiting for the one before.
 __device__ __forceinline__ void gelu_erf2x4(gelu_f32x2 (&x)[4]) {
     gelu_f32x2 relu[4], a[4], q[4];
 #pragma unroll
