@@ -1,0 +1,269 @@
+// Sums over the rows of every code, in a fixed order: what the gradient of a codeword lookup is, and the codebook gradient of
+// the quantiser's backward.  Float atomics would do it in one pass, but in the order of their arrival, and the codes of a
+// batch are used unevenly, so that the busiest codeword's adders queue.  Instead the rows are put in the order of their codes
+// (a stable radix sort of (code, row) pairs, 8 bytes each against the hundreds of bytes of a row) and walked in that order:
+//
+//   count      a histogram of the digit for every chunk of rows
+//   place      every chunk's pairs to their place: bin start + the bin's pairs of earlier chunks + rank within the chunk
+//              (two passes of up to 11 bits for more than 2047 codes, three beyond 4 million; one kernel that finds the runs)
+//   accumulate tiles of T sorted pairs, T the same for every tile however the codes are used; a group of lanes walks one tile and
+//              keeps the running sum in registers.  A code's run that lies within a tile is written at once; one that crosses
+//              tile borders leaves a partial sum on each
+//   join       the partial sums of a run in the order of the tiles, and zeros for codes without rows
+//
+// Up to kSmallRows rows all of it is one kernel (small): a workgroup owns a few codes, picks their rows out of all indices by
+// itself, in order, and sums them.
+//
+// An index outside [0, K) counts as the code K, which sorts last and has no sum.
+#pragma once
+#include "ckpt.h"
+
+namespace equss {
+
+struct IndexView {            // (num_pq, rows) indices of any integer type and any strides (in elements)
+    const void* p;
+    int type;                 // EQUSS_I64 / EQUSS_I32 / EQUSS_I16
+    int64_t stride_p, stride_r;
+};
+
+__device__ __forceinline__ uint32_t code_at(const IndexView& v, int p, int64_t r, uint32_t K) {
+    const int64_t at = (int64_t)p * v.stride_p + r * v.stride_r;
+    int64_t k;
+    if (v.type == EQUSS_I64) k = reinterpret_cast<const int64_t*>(v.p)[at];
+    else if (v.type == EQUSS_I32) k = reinterpret_cast<const int32_t*>(v.p)[at];
+    else k = reinterpret_cast<const int16_t*>(v.p)[at];
+    return k >= 0 && k < (int64_t)K ? (uint32_t)k : K;
+}
+
+struct CodePair { uint32_t code, row; };
+
+constexpr int kSmallRows = 2048;
+constexpr int kMaxBins = 2048;          // bins of a pass: 11 bits
+
+// What a call sorts with; everything but `index` lies in the caller's workspace.
+struct SortPlan {
+    int64_t rows;
+    int num_pq;
+    uint32_t K;
+    int passes, bits[3];
+    int chunks, chunk_rows;             // chunk_rows a multiple of 256
+    int tile;                           // T
+    int64_t tiles;
+    size_t pairs_a, pairs_b, table, starts, partial, total;   // byte offsets and the whole size
+};
+
+// d: elements of a row's part.  False where sizes pass what the kernels index with.
+bool sort_plan(SortPlan& s, int64_t rows, int num_pq, int64_t K, int d);
+// count / place (/ runs): afterwards the sorted pairs are at ws + the returned offset and starts at ws + s.starts
+int sort_launch(const SortPlan& s, const IndexView& index, char* ws, size_t* pairs_at, hipStream_t stream);
+
+// --------------------------------------------------------------------------------------------------------------------------
+// The walk.  Op gives the kernels their rows:
+//   struct Row;                                    what is loaded of one (row, p, lane)
+//   Row  load(row, p, col) const                   its loads
+//   struct Code; Code code(p, k, col) const        what it needs of the codeword (k == K: none)
+//   f32x4 value(const Row&, const Code&, row, p, col) const     the lane's four terms of the sum; may write the row's own output
+// A row's part of d elements is walked by LPR lanes with four elements each (d <= 4 LPR; beyond 256 in chunks of 256 columns).
+
+struct WalkArgs {
+    const CodePair* pairs;              // (num_pq, rows)
+    const uint32_t* starts;             // (num_pq, K + 1)
+    float* partial;                     // (num_pq, tiles, 2, dpad): a tile's head and tail
+    float* out;                         // (num_pq, K, d), or null: only the rows' own outputs are wanted
+    int64_t rows, tiles;
+    int tile, d, dpad;
+    uint32_t K;
+};
+
+__device__ __forceinline__ void store_cols(float* p, f32x4 v, int col, int d, bool whole) {
+    if (whole) *reinterpret_cast<f32x4*>(p) = v;          // (d a multiple of 4: 16-byte aligned)
+    else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (col + i < d) p[i] = v[i];
+    }
+}
+
+template <class Op, int LPR>
+__global__ __launch_bounds__(256) void code_accumulate_kernel(const Op op, const WalkArgs w) {
+    constexpr int SLOTS = 64 / LPR, U = 4;
+    const int lane = threadIdx.x & 63;
+    const int64_t tile = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * SLOTS + lane / LPR;
+    if (tile >= w.tiles) return;                          // (whole groups of LPR lanes leave together)
+    const int p = blockIdx.y, col = (int)blockIdx.z * 256 + (lane % LPR) * 4;
+    const bool live = col < w.d, whole = (w.d & 3) == 0;
+    const CodePair* pairs = w.pairs + (int64_t)p * w.rows;
+    const int64_t t0 = tile * w.tile, t1 = t0 + w.tile < w.rows ? t0 + w.tile : w.rows;
+    uint32_t cur = pairs[t0].code;
+    bool head = t0 > 0 && pairs[t0 - 1].code == cur;      // the run began in an earlier tile
+    float* part = w.partial + (((int64_t)p * w.tiles + tile) * 2) * w.dpad + col;
+    float* out = w.out + ((int64_t)p * w.K) * w.d + col;
+    const bool sums = w.out != nullptr;
+    typename Op::Code code = op.code(p, cur, live ? col : 0);
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int64_t i = t0; i < t1; i += U) {
+        CodePair pr[U];
+        typename Op::Row row[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) pr[j] = pairs[i + j < t1 ? i + j : t1 - 1];
+#pragma unroll
+        for (int j = 0; j < U; ++j) row[j] = op.load(pr[j].row, p, live ? col : 0);
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            if (i + j < t1) {
+                if (pr[j].code != cur) {
+                    if (sums && live && cur != w.K) {
+                        if (head) *reinterpret_cast<f32x4*>(part) = acc;
+                        else store_cols(out + (int64_t)cur * w.d, acc, col, w.d, whole);
+                    }
+                    head = false;
+                    cur = pr[j].code;
+                    code = op.code(p, cur, live ? col : 0);
+                    acc = f32x4{0.f, 0.f, 0.f, 0.f};
+                }
+                acc += op.value(row[j], code, pr[j].row, p, col, live);
+            }
+        }
+    }
+    if (sums && live && cur != w.K) {
+        const bool on = t1 < w.rows && pairs[t1].code == cur;
+        if (head) *reinterpret_cast<f32x4*>(part) = acc;
+        else if (on) *reinterpret_cast<f32x4*>(part + w.dpad) = acc;
+        else store_cols(out + (int64_t)cur * w.d, acc, col, w.d, whole);
+    }
+}
+
+// A wave owns a code; the chain of partial sums of a long run is shared by the workgroup's four waves.
+template <int LPR>
+__global__ __launch_bounds__(256) void code_join_kernel(const WalkArgs w) {
+    constexpr int SLOTS = 64 / LPR, kLong = 16 * SLOTS;
+    __shared__ f32x4 share[4 * 64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, slot = lane / LPR;
+    const int p = blockIdx.y, col = (int)blockIdx.z * 256 + (lane % LPR) * 4;
+    const bool live = col < w.d, whole = (w.d & 3) == 0;
+    const uint32_t* starts = w.starts + (int64_t)p * ((int64_t)w.K + 1);
+    const float* part = w.partial + (int64_t)p * w.tiles * 2 * w.dpad + (live ? col : 0);
+    float* out = w.out + (int64_t)p * w.K * w.d + col;
+    // link 0 is the first tile's tail, the others the following tiles' heads; sums of links first, first + step, ...
+    auto chain = [&](int64_t ts, int64_t links, int64_t first, int64_t step) {
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int64_t j = first; j < links; j += step)
+            acc += *reinterpret_cast<const f32x4*>(part + ((ts + j) * 2 + (j == 0 ? 1 : 0)) * w.dpad);
+        return acc;
+    };
+    const int64_t k0 = (int64_t)blockIdx.x * 4;
+    for (int c = 0; c < 4; ++c) {
+        const int64_t k = k0 + c;
+        if (k >= (int64_t)w.K) break;                      // (uniform over the workgroup)
+        const int64_t s = starts[k], e = starts[k + 1];
+        const int64_t ts = s / w.tile, links = e > s ? (e - 1) / w.tile - ts + 1 : 0;
+        const bool far = links > kLong;
+        if (!far) {
+            if (wave != c || links == 1) continue;         // one tile held the whole run: it is written already
+            f32x4 acc = chain(ts, links, slot, SLOTS);
+#pragma unroll
+            for (int o = 32; o >= LPR; o >>= 1)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], o, 64);
+            if (slot == 0 && live) store_cols(out + k * w.d, acc, col, w.d, whole);
+        } else {
+            share[wave * 64 + lane] = chain(ts, links, wave * SLOTS + slot, 4 * SLOTS);
+            __syncthreads();
+            if (wave == 0 && slot == 0 && live) {
+                f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+                for (int j = 0; j < 4 * SLOTS; ++j) acc += share[j * LPR + lane];
+                store_cols(out + k * w.d, acc, col, w.d, whole);
+            }
+            __syncthreads();
+        }
+    }
+}
+
+// All in one for few rows: the workgroup's codes are [k0, k0 + codes); `rest` tells the last workgroup to walk the rows
+// without a code too (for their own outputs).
+template <class Op, int LPR>
+__global__ __launch_bounds__(256) void code_small_kernel(const Op op, const IndexView index, float* __restrict__ out_all, int rows,
+                                                        uint32_t K, int d, int codes, int rest) {
+    constexpr int SLOTS = 256 / LPR;
+    __shared__ CodePair list[kSmallRows];
+    __shared__ f32x4 share[256];
+    __shared__ int wave_count[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, slot = tid / LPR;
+    const int p = blockIdx.y, col = (int)blockIdx.z * 256 + (tid % LPR) * 4;
+    const bool live = col < d, whole = (d & 3) == 0;
+    const uint32_t k0 = blockIdx.x * (uint32_t)codes;
+    uint32_t k1 = k0 + codes < K ? k0 + codes : K;
+    const uint32_t kend = k1;
+    if (rest && blockIdx.x == gridDim.x - 1) k1 = K + 1;
+    int count = 0;
+    for (int r0 = 0; r0 < rows; r0 += 256) {
+        const int r = r0 + tid;
+        uint32_t k = 0;
+        bool mine = false;
+        if (r < rows) {
+            k = code_at(index, p, r, K);
+            mine = k >= k0 && k < k1;
+        }
+        const uint64_t m = __ballot(mine);
+        if (lane == 0) wave_count[wave] = __popcll(m);
+        __syncthreads();
+        int at = count;
+        for (int i = 0; i < 4; ++i) {
+            if (i < wave) at += wave_count[i];
+            count += wave_count[i];
+        }
+        if (mine) list[at + __popcll(m & ((1ull << lane) - 1))] = CodePair{k, (uint32_t)r};
+        __syncthreads();
+    }
+    float* out = out_all + (int64_t)p * K * d + col;
+    const bool sums = out_all != nullptr;
+    const int lo = (int)((int64_t)count * slot / SLOTS), hi = (int)((int64_t)count * (slot + 1) / SLOTS);
+    for (uint32_t k = k0; k < k1; ++k) {
+        const typename Op::Code code = op.code(p, k, live ? col : 0);
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int j = lo; j < hi; ++j)
+            if (list[j].code == k) {
+                const uint32_t r = list[j].row;
+                acc += op.value(op.load(r, p, live ? col : 0), code, r, p, col, live);
+            }
+        if (!sums || k >= kend) continue;                  // (uniform)
+        share[tid] = acc;
+        __syncthreads();
+        if (slot == 0 && live) {
+            for (int j = 1; j < SLOTS; ++j) acc += share[j * LPR + tid];
+            store_cols(out + (int64_t)k * d, acc, col, d, whole);
+        }
+        __syncthreads();
+    }
+}
+
+template <class Op, int LPR>
+int walk_launch_lpr(const Op& op, const SortPlan& s, const IndexView& index, char* ws, float* out, int d, bool rest, hipStream_t stream) {
+    const unsigned cchunks = (unsigned)((d + 255) / 256);
+    if (s.passes == 0) {
+        // codes a workgroup: about a thousand workgroups
+        int64_t codes = ((int64_t)s.K * s.num_pq + 1023) / 1024;
+        if (codes < 1) codes = 1;
+        const unsigned gx = (unsigned)(((int64_t)s.K + codes - 1) / codes);
+        hipLaunchKernelGGL((code_small_kernel<Op, LPR>), dim3(gx, s.num_pq, cchunks), dim3(256), 0, stream, op, index, out, (int)s.rows, s.K,
+                           d, (int)codes, rest ? 1 : 0);
+        return check_launch("code_small_kernel");
+    }
+    size_t at = 0;
+    int rc = sort_launch(s, index, ws, &at, stream);
+    if (rc != EQUSS_OK) return rc;
+    WalkArgs w;
+    w.pairs = reinterpret_cast<const CodePair*>(ws + at);
+    w.starts = reinterpret_cast<const uint32_t*>(ws + s.starts);
+    w.partial = reinterpret_cast<float*>(ws + s.partial);
+    w.out = out; w.rows = s.rows; w.tiles = s.tiles; w.tile = s.tile; w.d = d; w.dpad = (d + 3) / 4 * 4; w.K = s.K;
+    constexpr int TILES_WG = 4 * (64 / LPR);
+    hipLaunchKernelGGL((code_accumulate_kernel<Op, LPR>), dim3((unsigned)((s.tiles + TILES_WG - 1) / TILES_WG), s.num_pq, cchunks), dim3(256), 0,
+                       stream, op, w);
+    rc = check_launch("code_accumulate_kernel");
+    if (rc != EQUSS_OK || !out) return rc;
+    hipLaunchKernelGGL((code_join_kernel<LPR>), dim3((s.K + 3) / 4, s.num_pq, cchunks), dim3(256), 0, stream, w);
+    return check_launch("code_join_kernel");
+}
+
+}  // namespace equss

@@ -1,0 +1,194 @@
+// The stable radix sort of (code, row) pairs behind the codeword sums: see code_sort.h.
+#include "code_sort.h"
+
+namespace {
+
+using equss::CodePair;
+using equss::IndexView;
+
+// first pass: the indices themselves; later ones: the pairs of the pass before
+struct Source {
+    IndexView index;
+    const CodePair* pairs;      // null in the first pass
+    int64_t rows;
+    uint32_t K;
+};
+
+__device__ __forceinline__ CodePair pair_at(const Source& s, int p, int64_t i) {
+    if (s.pairs) return s.pairs[(int64_t)p * s.rows + i];
+    return CodePair{equss::code_at(s.index, p, i, s.K), (uint32_t)i};
+}
+
+__global__ __launch_bounds__(256) void code_count_kernel(const Source s, uint32_t* __restrict__ table, int chunk_rows, int shift, int bits) {
+    __shared__ uint32_t hist[equss::kMaxBins];
+    const int bins = 1 << bits, p = blockIdx.y, chunk = blockIdx.x, chunks = gridDim.x;
+    for (int b = threadIdx.x; b < bins; b += 256) hist[b] = 0;
+    __syncthreads();
+    const int64_t i0 = (int64_t)chunk * chunk_rows, i1 = i0 + chunk_rows < s.rows ? i0 + chunk_rows : s.rows;
+    for (int64_t i = i0 + threadIdx.x; i < i1; i += 256) atomicAdd(&hist[(pair_at(s, p, i).code >> shift) & (bins - 1)], 1u);
+    __syncthreads();
+    uint32_t* row = table + ((int64_t)p * chunks + chunk) * bins;
+    for (int b = threadIdx.x; b < bins; b += 256) row[b] = hist[b];
+}
+
+// A wave owns a quarter of the chunk, so that ranks follow the row order.  starts: (num_pq, K + 1), written by the last pass of
+// one-pass sorts (whose bins are the codes), or null.
+__global__ __launch_bounds__(256) void code_place_kernel(const Source s, const uint32_t* __restrict__ table, CodePair* __restrict__ dst,
+                                                        uint32_t* __restrict__ starts, int chunk_rows, int shift, int bits) {
+    __shared__ uint32_t base[4][equss::kMaxBins];       // next place of every bin, for each wave
+    __shared__ uint32_t wave_sum[4];
+    const int bins = 1 << bits, p = blockIdx.y, chunk = blockIdx.x, chunks = gridDim.x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    for (int b = tid; b < 4 * bins; b += 256) base[b / bins][b % bins] = 0;
+    __syncthreads();
+    const int64_t i0 = (int64_t)chunk * chunk_rows + (int64_t)wave * (chunk_rows / 4);
+    int64_t i1 = i0 + chunk_rows / 4;
+    if (i1 > s.rows) i1 = s.rows;
+    for (int64_t i = i0 + lane; i < i1; i += 64) atomicAdd(&base[wave][(pair_at(s, p, i).code >> shift) & (bins - 1)], 1u);
+    __syncthreads();
+    // bins in runs of bins / 256 consecutive ones a thread, so that the exclusive sum over bins is one scan over threads
+    const int per = (bins + 255) / 256;
+    const uint32_t* rows_p = table + (int64_t)p * chunks * bins;
+    uint32_t before[equss::kMaxBins / 256], total[equss::kMaxBins / 256], sum = 0;
+#pragma unroll
+    for (int j = 0; j < equss::kMaxBins / 256; ++j) {
+        before[j] = total[j] = 0;
+        const int b = tid * per + j;
+        if (j < per && b < bins) {
+            for (int c = 0; c < chunks; ++c) {
+                const uint32_t n = rows_p[(int64_t)c * bins + b];
+                if (c < chunk) before[j] += n;
+                total[j] += n;
+            }
+            sum += total[j];
+        }
+    }
+    uint32_t scan = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t up = (uint32_t)__shfl_up((int)scan, o, 64);
+        if (lane >= o) scan += up;
+    }
+    if (lane == 63) wave_sum[wave] = scan;
+    __syncthreads();
+    uint32_t start = scan - sum;
+    for (int i = 0; i < wave; ++i) start += wave_sum[i];
+#pragma unroll
+    for (int j = 0; j < equss::kMaxBins / 256; ++j) {
+        const int b = tid * per + j;
+        if (j < per && b < bins) {
+            if (starts && chunk == 0 && (uint32_t)b <= s.K) starts[(int64_t)p * ((int64_t)s.K + 1) + b] = start;
+            uint32_t at = start + before[j];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const uint32_t n = base[v][b];
+                base[v][b] = at;
+                at += n;
+            }
+            start += total[j];
+        }
+    }
+    __syncthreads();
+    // 64 pairs at a time: lanes of equal digit find each other by one ballot a bit; their rank is the number of such lanes below
+    CodePair* out = dst + (int64_t)p * s.rows;
+    for (int64_t i = i0; i < i1; i += 64) {
+        const bool in = i + lane < i1;
+        CodePair pr = {0, 0};
+        if (in) pr = pair_at(s, p, i + lane);
+        const uint32_t digit = (pr.code >> shift) & (bins - 1);
+        uint64_t same = __ballot(in);
+        for (int b = 0; b < bits; ++b) {
+            const uint64_t set = __ballot((digit >> b) & 1);
+            same &= (digit >> b) & 1 ? set : ~set;
+        }
+        if (in) {
+            const uint32_t rank = __popcll(same & ((1ull << lane) - 1));
+            // (all lanes read before the first of them writes: LDS operations of a wave stay in order)
+            const uint32_t at = __hip_atomic_load(&base[wave][digit], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+            if (rank == 0) __hip_atomic_store(&base[wave][digit], at + (uint32_t)__popcll(same), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+            out[at + rank] = pr;
+        }
+    }
+}
+
+// where every code's run starts among the sorted pairs: the first pair whose code is not below it
+__global__ __launch_bounds__(256) void code_runs_kernel(const CodePair* __restrict__ pairs, uint32_t* __restrict__ starts, int64_t rows, uint32_t K) {
+    const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (k > (int64_t)K) return;
+    const CodePair* pp = pairs + (int64_t)blockIdx.y * rows;
+    int64_t lo = 0, hi = rows;
+    while (lo < hi) {
+        const int64_t mid = (lo + hi) >> 1;
+        if ((int64_t)pp[mid].code < k) lo = mid + 1;
+        else hi = mid;
+    }
+    starts[(int64_t)blockIdx.y * ((int64_t)K + 1) + k] = (uint32_t)lo;
+}
+
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+}  // namespace
+
+namespace equss {
+
+bool sort_plan(SortPlan& s, int64_t rows, int num_pq, int64_t K, int d) {
+    s = SortPlan{};
+    s.rows = rows;
+    s.num_pq = num_pq;
+    s.K = (uint32_t)K;
+    if (rows > 0x7fffff00 || num_pq > 65535 || K >= ((int64_t)1 << 31)) return false;
+    if (rows <= kSmallRows) return true;                   // one kernel, no workspace
+    int bits = 1;
+    while (((int64_t)1 << bits) <= K) ++bits;              // values 0 .. K
+    s.passes = (bits + 10) / 11;
+    for (int i = 0, left = bits; i < s.passes; ++i) {
+        s.bits[i] = (left + s.passes - i - 1) / (s.passes - i);
+        left -= s.bits[i];
+    }
+    int64_t chunk = (rows + 63) / 64;                      // at most 64 chunks: every one reads the others' counts
+    if (chunk < 2048) chunk = 2048;
+    s.chunk_rows = (int)((chunk + 255) / 256 * 256);
+    s.chunks = (int)((rows + s.chunk_rows - 1) / s.chunk_rows);
+    s.tile = 64;
+    s.tiles = (rows + s.tile - 1) / s.tile;
+    size_t at = 0;
+    const size_t pairs = align256((size_t)num_pq * rows * sizeof(CodePair));
+    s.pairs_a = at; at += pairs;
+    s.pairs_b = at; at += s.passes > 1 ? pairs : 0;
+    s.table = at; at += align256((size_t)num_pq * s.chunks * kMaxBins * sizeof(uint32_t));
+    s.starts = at; at += align256((size_t)num_pq * (K + 1) * sizeof(uint32_t));
+    s.partial = at; at += align256((size_t)num_pq * s.tiles * 2 * ((d + 3) / 4 * 4) * sizeof(float));
+    s.total = at;
+    return true;
+}
+
+int sort_launch(const SortPlan& s, const IndexView& index, char* ws, size_t* pairs_at, hipStream_t stream) {
+    Source src;
+    src.index = index; src.pairs = nullptr; src.rows = s.rows; src.K = s.K;
+    uint32_t* table = reinterpret_cast<uint32_t*>(ws + s.table);
+    uint32_t* starts = reinterpret_cast<uint32_t*>(ws + s.starts);
+    const dim3 grid((unsigned)s.chunks, (unsigned)s.num_pq);
+    size_t dst = s.pairs_a;
+    int shift = 0;
+    for (int i = 0; i < s.passes; ++i) {
+        dst = (i & 1) ? s.pairs_b : s.pairs_a;
+        hipLaunchKernelGGL(code_count_kernel, grid, dim3(256), 0, stream, src, table, s.chunk_rows, shift, s.bits[i]);
+        int rc = check_launch("code_count_kernel");
+        if (rc != EQUSS_OK) return rc;
+        hipLaunchKernelGGL(code_place_kernel, grid, dim3(256), 0, stream, src, table, reinterpret_cast<CodePair*>(ws + dst),
+                           s.passes == 1 ? starts : nullptr, s.chunk_rows, shift, s.bits[i]);
+        rc = check_launch("code_place_kernel");
+        if (rc != EQUSS_OK) return rc;
+        shift += s.bits[i];
+        src.pairs = reinterpret_cast<const CodePair*>(ws + dst);
+    }
+    *pairs_at = dst;
+    if (s.passes > 1) {
+        hipLaunchKernelGGL(code_runs_kernel, dim3((unsigned)(((int64_t)s.K + 1 + 255) / 256), (unsigned)s.num_pq), dim3(256), 0, stream, src.pairs, starts,
+                           s.rows, s.K);
+        return check_launch("code_runs_kernel");
+    }
+    return EQUSS_OK;
+}
+
+}  // namespace equss

@@ -61,6 +61,11 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2_t));
 }
 
+// The bits of one 32-bit value as another type, by value: __builtin_bit_cast applied to a vector's element (v[i], which is an
+// lvalue) takes the vector's first element whatever i is.
+template <class To>
+__device__ __forceinline__ To bits_as(uint32_t w) { return __builtin_bit_cast(To, w); }
+
 // GELU (erf form, torch.nn.GELU's default) with one transcendental:
 //   gelu(x) = x * Phi(x) = max(x, 0) - |x| * (erfc(|x| / sqrt 2) / 2),   erfc(|x| / sqrt 2) / 2 = 2^Q(|x|),
 // Q a degree-5 polynomial fitted to log2 of that tail (smooth and nearly quadratic, unlike erf itself),

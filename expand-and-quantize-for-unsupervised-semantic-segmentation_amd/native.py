@@ -32,6 +32,8 @@ EXPORTED_SYMBOLS = [
     "equss_vit_f32_workspace_bytes", "equss_vit_forward_f32", "equss_expand_head_f32",
     "equss_probe_workspace_bytes", "equss_probe_eval", "equss_probe_train", "equss_confusion_update", "equss_pq_st_backward", "equss_gemm_tn_bf16", "equss_tap_gather", "equss_tap_scatter",
     "equss_index_rows_i16", "equss_code_usage",
+    "equss_ckpt_pack", "equss_ckpt_unpack", "equss_gemm_tn_ckpt_workspace_bytes", "equss_gemm_tn_ckpt",
+    "equss_pq_st_backward_ckpt", "equss_code_lookup", "equss_code_sums_sorted_workspace_bytes", "equss_code_lookup_grad",
 ]
 
 
@@ -142,6 +144,25 @@ def _declare(lib):
     lib.equss_pq_st_backward.restype = c_int
     lib.equss_pq_st_backward.argtypes = [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, ctypes.c_float, ctypes.c_float,
                                          c_vp, c_i64, c_vp, c_int, c_int, c_int, c_int, c_vp]
+    lib.equss_ckpt_pack.restype = c_int
+    lib.equss_ckpt_pack.argtypes = [c_vp, c_int, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_int, c_int, c_int, c_vp]
+    lib.equss_ckpt_unpack.restype = c_int
+    lib.equss_ckpt_unpack.argtypes = [c_vp, c_i64, c_vp, c_i64, c_vp, c_int, c_i64, c_i64, c_int, c_int, c_vp]
+    lib.equss_gemm_tn_ckpt_workspace_bytes.restype = c_sz
+    lib.equss_gemm_tn_ckpt_workspace_bytes.argtypes = [c_i64, c_int, c_int]
+    lib.equss_gemm_tn_ckpt.restype = c_int
+    lib.equss_gemm_tn_ckpt.argtypes = [c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_int, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_int,
+                                       c_int, c_vp, c_sz, c_vp]
+    lib.equss_pq_st_backward_ckpt.restype = c_int
+    lib.equss_pq_st_backward_ckpt.argtypes = [c_vp, c_i64, c_vp, c_i64, c_int, c_vp, c_vp, c_vp, c_i64, c_vp, c_f, c_f, c_vp, c_i64,
+                                              c_vp, c_i64, c_int, c_int, c_int, c_vp, c_sz, c_vp]
+    lib.equss_code_lookup.restype = c_int
+    lib.equss_code_lookup.argtypes = [c_vp, c_int, c_i64, c_i64, c_vp, c_int, c_f, c_vp, c_i64, c_i64, c_int, c_i64, c_int, c_vp]
+    lib.equss_code_sums_sorted_workspace_bytes.restype = c_sz
+    lib.equss_code_sums_sorted_workspace_bytes.argtypes = [c_i64, c_int, c_i64, c_int]
+    lib.equss_code_lookup_grad.restype = c_int
+    lib.equss_code_lookup_grad.argtypes = [c_vp, c_int, c_i64, c_vp, c_int, c_i64, c_i64, c_f, c_vp, c_i64, c_int, c_i64, c_int, c_vp,
+                                           c_sz, c_vp]
     lib.equss_probe_eval.restype = c_int
     lib.equss_probe_eval.argtypes = [c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_sz,
                                      c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_vp]
@@ -637,6 +658,207 @@ def pq_st_backward(rows, emb, idx, g_zq, g_vq, beta, book, num_codes, d, want_ro
                                     _ptr(g_rows), g_rows.stride(0) if want_rows else 0, _ptr(g_books), n, num_pq,
                                     num_codes, d, _stream(rows)), "equss_pq_st_backward")
     return g_rows, g_books
+
+
+# ------------------------------------------------------------------------------------------------
+# 8-bit activation checkpoints and the codeword lookup
+# ------------------------------------------------------------------------------------------------
+CKPT_BLOCK = 32                      # channels that share a scale
+CKPT_FORMATS = {"int8": 0, "e4m3": 1}
+_CKPT_DTYPES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+_ELEM_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_INDEX_TYPES = {torch.int64: 0, torch.int32: 1, torch.int16: 2}
+
+
+class ActCheckpoint:
+    """An activation (rows, width) kept in 8 bits: ``codes`` (rows, width rounded up to whole blocks of 32) int8 or
+    float8_e4m3fn, ``scales`` (rows, blocks) uint8, a block's value being code * 2^(scale - 127) (scale 255: a block that held
+    an infinity or a NaN, NaN throughout).  Made by ``ckpt_pack``; the two tensors are all there is to save or move."""
+
+    __slots__ = ("codes", "scales", "width")
+
+    def __init__(self, codes, scales, width):
+        blocks = (width + CKPT_BLOCK - 1) // CKPT_BLOCK
+        if codes.dtype not in _CKPT_DTYPES.values() or codes.dim() != 2 or width <= 0 or codes.shape[1] != blocks * CKPT_BLOCK:
+            raise ValueError(f"ActCheckpoint: codes must be (rows, {blocks * CKPT_BLOCK}) int8 or float8_e4m3fn for width {width}")
+        if scales.dtype != torch.uint8 or scales.shape != (codes.shape[0], blocks) or scales.device != codes.device:
+            raise ValueError(f"ActCheckpoint: scales must be ({codes.shape[0]}, {blocks}) uint8 beside the codes")
+        self.codes, self.scales, self.width = codes, scales, width
+
+    @property
+    def rows(self):
+        return self.codes.shape[0]
+
+    @property
+    def fmt(self):
+        return "int8" if self.codes.dtype == torch.int8 else "e4m3"
+
+    def columns(self, start, stop):
+        """The checkpoint of columns [start, stop) as views; start a multiple of 32, stop too unless it is the width."""
+        if not 0 <= start < stop <= self.width or start % CKPT_BLOCK or (stop % CKPT_BLOCK and stop != self.width):
+            raise ValueError(f"columns [{start}, {stop}) of a checkpoint of {self.width} do not lie on blocks of {CKPT_BLOCK}")
+        last = (stop + CKPT_BLOCK - 1) // CKPT_BLOCK
+        return ActCheckpoint(self.codes[:, start:last * CKPT_BLOCK], self.scales[:, start // CKPT_BLOCK:last], stop - start)
+
+
+def _row_major(t):
+    """(t or a copy with unit column stride and rows that do not overlap, leading dimension)."""
+    rows, width = t.shape
+    if (width > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < width):
+        t = t.contiguous()
+    return t, (t.stride(0) if rows > 1 else max(width, 1))
+
+
+def _ckpt_parts(ckpt):
+    """Pointers and leading dimensions of a checkpoint in the layout the kernels take (column views included)."""
+    codes, scales = ckpt.codes, ckpt.scales
+    if codes.shape[0] > 1 and (codes.stride(1) != 1 or codes.stride(0) % CKPT_BLOCK or codes.stride(0) < codes.shape[1]) or codes.data_ptr() % 16:
+        codes = codes.clone(memory_format=torch.contiguous_format)
+    scales, ld_scales = _row_major(scales)
+    return codes, (codes.stride(0) if codes.shape[0] > 1 else codes.shape[1]), scales, ld_scales
+
+
+def _same_device(*ts):
+    _need_cuda(*ts)
+    if len({t.device for t in ts if t is not None}) > 1:
+        raise ValueError("all tensors of a call must be on one device")
+
+
+def ckpt_pack(x, fmt="int8", keep_sign=False):
+    """x (rows, width) fp32 / bf16 / fp16 -> ActCheckpoint in ``fmt`` "int8" or "e4m3": one byte a value and one for 32
+    consecutive channels.  ``keep_sign``: a value other than zero never becomes zero, so that ``code > 0`` is the mask of a
+    ReLU whose result is kept (see equss_ckpt_pack in the header for the rounding)."""
+    _need_cuda(x)
+    if fmt not in CKPT_FORMATS:
+        raise ValueError(f"Unsupported checkpoint format {fmt}")
+    if x.dim() != 2 or x.dtype not in _ELEM_TYPES or x.shape[1] == 0:
+        raise ValueError("ckpt_pack: x must be a (rows, width) float32, bfloat16 or float16 tensor")
+    x, ld = _row_major(x)
+    rows, width = x.shape
+    blocks = (width + CKPT_BLOCK - 1) // CKPT_BLOCK
+    codes = torch.empty((rows, blocks * CKPT_BLOCK), dtype=_CKPT_DTYPES[fmt], device=x.device)
+    scales = torch.empty((rows, blocks), dtype=torch.uint8, device=x.device)
+    _check(load_library().equss_ckpt_pack(_ptr(x), _ELEM_TYPES[x.dtype], ld, _ptr(codes), blocks * CKPT_BLOCK, _ptr(scales), blocks, rows,
+                                          width, CKPT_FORMATS[fmt], int(bool(keep_sign)), _stream(x)), "equss_ckpt_pack")
+    return ActCheckpoint(codes, scales, width)
+
+
+def ckpt_unpack(ckpt, dtype=torch.float32):
+    """The kept values (rows, width) in fp32, bf16 or fp16 (exact in the first two)."""
+    _same_device(ckpt.codes, ckpt.scales)
+    if dtype not in _ELEM_TYPES:
+        raise ValueError("ckpt_unpack: dtype must be float32, bfloat16 or float16")
+    codes, ld_codes, scales, ld_scales = _ckpt_parts(ckpt)
+    out = torch.empty((ckpt.rows, ckpt.width), dtype=dtype, device=codes.device)
+    _check(load_library().equss_ckpt_unpack(_ptr(codes), ld_codes, _ptr(scales), ld_scales, _ptr(out), _ELEM_TYPES[dtype], ckpt.width,
+                                            ckpt.rows, ckpt.width, CKPT_FORMATS[ckpt.fmt], _stream(codes)), "equss_ckpt_unpack")
+    return out
+
+
+def gemm_tn_ckpt(a, ckpt, relu=None, want_bias=False):
+    """a (rows, M) bf16, ckpt the kept input (rows, N) of a linear layer -> a^T V (M, N) fp32, the weight gradient; with
+    ``want_bias`` also the column sums of a (M,) fp32.  ``relu``: checkpoint (rows, M) of the layer's output behind a ReLU
+    (packed with keep_sign): a counts only where it is positive.  Sums in a fixed order."""
+    _same_device(a, ckpt.codes, ckpt.scales, relu.codes if relu is not None else None)
+    if a.dtype != torch.bfloat16 or a.dim() != 2 or a.shape[0] != ckpt.rows or a.shape[1] == 0:
+        raise ValueError(f"gemm_tn_ckpt: a must be a ({ckpt.rows}, M) bfloat16 tensor")
+    rows, m = a.shape
+    if relu is not None and (relu.rows != rows or relu.width != m):
+        raise ValueError(f"gemm_tn_ckpt: the ReLU checkpoint must be ({rows}, {m}), is ({relu.rows}, {relu.width})")
+    a, lda = _row_major(a)
+    codes, ld_codes, scales, ld_scales = _ckpt_parts(ckpt)
+    mask, ld_mask = _ckpt_parts(relu)[:2] if relu is not None else (None, 0)
+    out = torch.empty((m, ckpt.width), dtype=torch.float32, device=a.device)
+    bias = torch.empty((m,), dtype=torch.float32, device=a.device) if want_bias else None
+    lib = load_library()
+    # (scratch is allocated for the call, not kept: a call captured into a graph then holds its own)
+    nbytes = lib.equss_gemm_tn_ckpt_workspace_bytes(rows, m, ckpt.width)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=a.device) if nbytes else None
+    _check(lib.equss_gemm_tn_ckpt(_ptr(a), lda, _ptr(codes), ld_codes, _ptr(scales), ld_scales, CKPT_FORMATS[ckpt.fmt], _ptr(mask), ld_mask,
+                                  _ptr(out), ckpt.width, _ptr(bias), rows, m, ckpt.width, _ptr(ws), nbytes, _stream(a)),
+           "equss_gemm_tn_ckpt")
+    return (out, bias) if want_bias else out
+
+
+def pq_st_backward_ckpt(ckpt, books, idx, g_zq, g_vq, beta, book, want_rows=True, want_books=True):
+    """pq_st_backward from the 8-bit checkpoint (n, num_pq*d) of the codes and the codebooks (num_pq, K, d) fp32 themselves:
+    idx (num_pq, n) int64, g_zq (n, num_pq*d) or None, g_vq a 0-dim tensor -> (g_rows or None, g_books or None)."""
+    _same_device(ckpt.codes, ckpt.scales, books, idx, g_zq, g_vq)
+    if books.dim() != 3 or books.dtype != torch.float32:
+        raise ValueError("pq_st_backward_ckpt: books must be a (num_pq, K, d) float32 tensor")
+    num_pq, k, d = books.shape
+    n = ckpt.rows
+    if ckpt.width != num_pq * d:
+        raise ValueError(f"pq_st_backward_ckpt: the checkpoint has {ckpt.width} channels, the codebooks need {num_pq}x{d}")
+    if idx.dtype != torch.int64 or idx.shape != (num_pq, n):
+        raise ValueError(f"pq_st_backward_ckpt: idx must be ({num_pq}, {n}) int64")
+    if g_zq is not None:
+        if g_zq.shape != (n, num_pq * d):
+            raise ValueError(f"pq_st_backward_ckpt: g_zq must be ({n}, {num_pq * d})")
+        g_zq = g_zq.float()
+        if (n > 1 and (g_zq.stride(0) < num_pq * d or g_zq.stride(0) % 4)) or g_zq.stride(1) != 1 or g_zq.data_ptr() % 16:
+            g_zq = g_zq.clone(memory_format=torch.contiguous_format)
+    codes, ld_codes, scales, ld_scales = _ckpt_parts(ckpt)
+    books = books.contiguous()
+    if books.data_ptr() % 16:
+        books = books.clone()
+    idx = idx.contiguous()
+    g_vq = g_vq.reshape(1).float().contiguous()
+    dev = books.device
+    g_rows = torch.empty((n, num_pq * d), dtype=torch.float32, device=dev) if want_rows else None
+    g_books = torch.empty((num_pq, k, d), dtype=torch.float32, device=dev) if want_books else None
+    lib = load_library()
+    nbytes = lib.equss_code_sums_sorted_workspace_bytes(n, num_pq, k, d)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _check(lib.equss_pq_st_backward_ckpt(_ptr(codes), ld_codes, _ptr(scales), ld_scales, CKPT_FORMATS[ckpt.fmt], _ptr(books), _ptr(idx),
+                                         _ptr(g_zq), (g_zq.stride(0) if n > 1 else num_pq * d) if g_zq is not None else 0, _ptr(g_vq),
+                                         float(beta), float(book), _ptr(g_rows), num_pq * d, _ptr(g_books), n, num_pq, k, d, _ptr(ws), nbytes,
+                                         _stream(books)), "equss_pq_st_backward_ckpt")
+    return g_rows, g_books
+
+
+def _index_args(idx, what):
+    if idx.dim() != 2 or idx.dtype not in _INDEX_TYPES:
+        raise ValueError(f"{what}: idx must be a (num_pq, rows) int64, int32 or int16 tensor")
+    return _ptr(idx), _INDEX_TYPES[idx.dtype], idx.stride(0), idx.stride(1)
+
+
+def code_lookup(idx, books, scale=1.0):
+    """idx (num_pq, rows) int64 / int32 / int16 of any strides (an index dump's rows are ``rows.t()``), books (num_pq, K, d)
+    fp32 / bf16 / fp16 -> (rows, num_pq*d) of the books' type: scale * books[p, idx[p, r]], zeros where the index lies outside
+    [0, K)."""
+    _same_device(idx, books)
+    if books.dim() != 3 or books.dtype not in _ELEM_TYPES or idx.dim() != 2 or books.shape[0] != idx.shape[0]:
+        raise ValueError("code_lookup: books must be (num_pq, K, d) float32, bfloat16 or float16 with as many sub-spaces as idx")
+    num_pq, k, d = books.shape
+    where = _index_args(idx, "code_lookup")
+    rows = idx.shape[1]
+    books = books.contiguous()
+    if books.data_ptr() % 16:
+        books = books.clone()
+    out = torch.empty((rows, num_pq * d), dtype=books.dtype, device=books.device)
+    _check(load_library().equss_code_lookup(*where, _ptr(books), _ELEM_TYPES[books.dtype], float(scale), _ptr(out), num_pq * d, rows, num_pq,
+                                            k, d, _stream(books)), "equss_code_lookup")
+    return out
+
+
+def code_lookup_grad(g, idx, num_codes, scale=1.0):
+    """The gradient of code_lookup: g (rows, num_pq*d) fp32 / bf16 / fp16, idx (num_pq, rows) as there -> (num_pq, num_codes, d)
+    fp32, scale times the sum of every codeword's rows, in a fixed order."""
+    _same_device(g, idx)
+    where = _index_args(idx, "code_lookup_grad")
+    num_pq, rows = idx.shape
+    if g.dim() != 2 or g.dtype not in _ELEM_TYPES or g.shape[0] != rows or num_pq == 0 or g.shape[1] == 0 or g.shape[1] % num_pq:
+        raise ValueError(f"code_lookup_grad: g must be a ({rows}, {num_pq}*d) float32, bfloat16 or float16 tensor")
+    d = g.shape[1] // num_pq
+    g, ld = _row_major(g)
+    out = torch.empty((num_pq, num_codes, d), dtype=torch.float32, device=g.device)
+    lib = load_library()
+    nbytes = lib.equss_code_sums_sorted_workspace_bytes(rows, num_pq, int(num_codes), d)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=g.device) if nbytes else None
+    _check(lib.equss_code_lookup_grad(_ptr(g), _ELEM_TYPES[g.dtype], ld, *where, float(scale), _ptr(out), rows, num_pq, int(num_codes), d,
+                                      _ptr(ws), nbytes, _stream(g)), "equss_code_lookup_grad")
+    return out
 
 
 def probe_train(feat_rows, probes, bias, label, batch, h, w, n_linear, n_cluster):

@@ -52,6 +52,13 @@ enum {
     EQUSS_EPI_RESID_F32 = 4   /* out_f32 += acc + bias  (residual, vision_transformer.py:110-111) */
 };
 
+/* element types of the entry points that take several */
+enum { EQUSS_F32 = 0, EQUSS_BF16 = 1, EQUSS_F16 = 2 };
+/* index types of equss_code_lookup / equss_code_lookup_grad */
+enum { EQUSS_I64 = 0, EQUSS_I32 = 1, EQUSS_I16 = 2 };
+/* formats of an 8-bit activation checkpoint (equss_ckpt_pack) */
+enum { EQUSS_CKPT_INT8 = 0, EQUSS_CKPT_E4M3 = 1 };
+
 int equss_abi_version(void);
 const char* equss_last_error(void);
 
@@ -403,6 +410,70 @@ int equss_pq_st_backward(const float* z, int64_t ld_z, const float* emb, int64_t
  *   place (clear it first).  Float atomic adds: equal to the matrix product to rounding, not bit for bit. */
 int equss_code_sums(const float* z, int64_t ld_z, const int64_t* idx, float* sums, int64_t rows, int num_pq, int K, int d,
                     void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * 8-bit activation checkpoints: what a backward pass needs of the forward, kept in one byte a value plus one scale byte for 32
+ * consecutive channels of a row (the last block of a row may be shorter).  Scale byte b stands for 2^(b - 127).  Of a block with
+ * largest magnitude A, the scale is 2^k with the smallest integer k >= -110 for which A 2^-k, rounded to the format, does not
+ * pass its largest value (int8: 127, e4m3: 448); a code is x 2^-k rounded to nearest even, off by half a step of the format at
+ * most.  Nothing saturates, and every kept value is exact in bf16 and fp32.  A block that holds an infinity or a NaN gets scale
+ * byte 255 and codes 0 and reads back as NaN throughout.
+ *   keep_sign != 0: a value other than zero that would round to zero becomes the smallest code of its sign instead (off by less
+ *            than one such step), so that "code > 0" is the mask of a ReLU whose result is kept
+ *   x / out  (rows, width), type EQUSS_F32 / _BF16 / _F16, unit column stride, leading dimension in elements, any alignment
+ *   codes    (rows, ld_codes) bytes out / in, 16-byte aligned, ld_codes a multiple of 32, >= width rounded up to 32 (the padding
+ *            is written as zero codes); scales (rows, ld_scales) bytes, one for each block of 32
+ * Both launch one kernel; rows == 0 launches none.  width <= 524288.
+ * ------------------------------------------------------------------------------------------- */
+int equss_ckpt_pack(const void* x, int type, int64_t ld_x, void* codes, int64_t ld_codes, void* scales, int64_t ld_scales,
+                    int64_t rows, int width, int fmt, int keep_sign, void* stream);
+int equss_ckpt_unpack(const void* codes, int64_t ld_codes, const void* scales, int64_t ld_scales, void* out, int type,
+                      int64_t ld_out, int64_t rows, int width, int fmt, void* stream);
+
+/* Weight and bias gradient of a linear layer (the backward of model/dino_pqgo.py:104-112) whose input V was kept by
+ * equss_ckpt_pack:  C[m][n] = sum over r < rows of a[r][m] V[r][n],  bias[m] = sum over r of a[r][m].
+ *   a      (rows, M) bf16, leading dimension lda, any alignment
+ *   codes, scales, fmt: V (rows, N) as equss_ckpt_pack wrote it
+ *   relu_codes (rows, M) codes of a checkpoint of either format, or NULL: a[r][m] counts only where the code is > 0, in both sums
+ *   C      (M, N) fp32 out, leading dimension ldc; bias (M) fp32 out or NULL
+ *   workspace equss_gemm_tn_ckpt_workspace_bytes() bytes, 16-byte aligned (may be NULL where that is 0)
+ * M, N and rows are any size (rows == 0 gives zeros).  bf16 MFMA on exactly the kept values, fp32 accumulation; the partial sums
+ * of the row ranges are added in a fixed order: equal calls give equal bits. */
+size_t equss_gemm_tn_ckpt_workspace_bytes(int64_t rows, int M, int N);
+int equss_gemm_tn_ckpt(const void* a, int64_t lda, const void* codes, int64_t ld_codes, const void* scales, int64_t ld_scales,
+                       int fmt, const void* relu_codes, int64_t ld_relu, float* C, int64_t ldc, float* bias, int64_t rows, int M,
+                       int N, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Backward of the training-pass quantisation as equss_pq_st_backward, with the codes z kept by equss_ckpt_pack and the
+ * codewords taken from the codebooks:
+ *   codes, scales, fmt: z (rows, num_pq*d); books (num_pq, K, d) fp32; idx (num_pq, rows) int64
+ *   g_zq, g_vq, g_z, g_books, beta, book: as equss_pq_st_backward
+ *   workspace equss_code_sums_sorted_workspace_bytes() bytes, 256-byte aligned (may be NULL where that is 0)
+ * An index outside [0, K) is taken for a codeword of zeros and adds to no codeword's gradient.  The rows of a codeword are summed
+ * in a fixed order: equal calls give equal bits.  d in {16, 32, 64, 128}; float buffers 16-byte aligned. */
+int equss_pq_st_backward_ckpt(const void* codes, int64_t ld_codes, const void* scales, int64_t ld_scales, int fmt,
+                              const float* books, const int64_t* idx, const float* g_zq, int64_t ld_g, const float* g_vq,
+                              float beta, float book, float* g_z, int64_t ld_gz, float* g_books, int64_t rows, int num_pq, int K,
+                              int d, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Codewords by their indices (the gather of model/dino_pqgo.py:659-663 on its own: indices, an index dump's rows say, back to
+ * features), with a scale:  out[r][p*d + j] = scale * books[p][idx[p][r]][j], and zeros where the index lies outside [0, K)
+ * (-1 marks a place without a token).
+ *   idx   (num_pq, rows) of index_type EQUSS_I64 / _I32 / _I16, element (p, r) at idx[p*stride_p + r*stride_r]
+ *   books (num_pq, K, d) of type EQUSS_F32 / _BF16 / _F16, 16-byte aligned; out (rows, num_pq*d) of the same type, any alignment
+ * The product is taken in fp32 and rounded once. */
+int equss_code_lookup(const void* idx, int index_type, int64_t stride_p, int64_t stride_r, const void* books, int type,
+                      float scale, void* out, int64_t ld_out, int64_t rows, int num_pq, int64_t K, int d, void* stream);
+
+/* Its gradient:  g_books[p][k][j] = scale * sum over r with idx[p][r] == k of g[r][p*d + j].
+ *   g (rows, num_pq*d) of type EQUSS_F32 / _BF16 / _F16, any alignment; g_books (num_pq, K, d) fp32 out, 16-byte aligned, written
+ *   whole (codes without rows get zeros; indices outside [0, K) add to none)
+ *   workspace equss_code_sums_sorted_workspace_bytes() bytes, 256-byte aligned (may be NULL where that is 0)
+ * fp32 sums in a fixed order: equal calls give equal bits.  rows < 2^31 - 256. */
+size_t equss_code_sums_sorted_workspace_bytes(int64_t rows, int num_pq, int64_t K, int d);
+int equss_code_lookup_grad(const void* g, int type, int64_t ld_g, const void* idx, int index_type, int64_t stride_p,
+                           int64_t stride_r, float scale, float* g_books, int64_t rows, int num_pq, int64_t K, int d,
+                           void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
