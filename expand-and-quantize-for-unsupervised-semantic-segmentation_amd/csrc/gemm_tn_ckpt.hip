@@ -31,7 +31,7 @@ struct Args {
     int64_t split_c;
     float* bias; int64_t split_bias;           // or null
     int64_t rows, rows_split;
-    int M, N, tiles_m, tiles_n, npad, mpad;
+    int M, N, tiles_m, tiles_n, splits, npad, mpad;
 };
 
 template <bool E4M3, bool MASK>
@@ -187,42 +187,256 @@ __global__ __launch_bounds__(kTnThreads, 2) void gemm_tn_ckpt_kernel(const Args 
     }
 }
 
+// ---- the large tile: 4 waves, WM x WN MFMA tiles of 32 x 32 each, i.e. 64 WM x 64 WN of C; 64 rows a stage, two stages in LDS.
+// A wave's accumulators take up to 256 registers, so one wave a SIMD; what hides its latencies is its own pipeline: while it
+// multiplies stage s out of LDS, the registers hold stage s + 1 (requested a whole stage earlier), which goes through the
+// conversion into the other half of LDS a quarter at a time, each quarter's registers being refilled at once from stage s + 2.
+// Columns past M: the last chunk of 8 columns is read at M - 8, so that every load is whole and inside; the chunk's columns
+// then overlap the chunk before, both give the same sums, and both are written.  Columns past N lie in the checkpoint's
+// padding or are read from its last block; their sums are dropped.
+constexpr int kBigBK = 64;
+
+template <int T64> struct TileRow { static constexpr int bytes = T64 == 2 ? 256 : 512; };   // (192 columns in rows of 512: the swizzle's xor needs them)
+
+template <bool E4M3>
+__device__ __forceinline__ u32x4a to_bf16x8(uint32_t c0, uint32_t c1, float s) {
+    const f32x4 lo = equss::ckpt_decode4<E4M3>(c0), hi = equss::ckpt_decode4<E4M3>(c1);
+    return u32x4a{equss::pack_bf16(lo[0] * s, lo[1] * s), equss::pack_bf16(lo[2] * s, lo[3] * s),
+                  equss::pack_bf16(hi[0] * s, hi[1] * s), equss::pack_bf16(hi[2] * s, hi[3] * s)};
+}
+
+template <bool E4M3, bool MASK, int WM, int WN>
+__global__ __launch_bounds__(256, 1) void gemm_tn_ckpt_big_kernel(const Args g) {
+    constexpr int TMB = 64 * WM, TNB = 64 * WN, RA = TileRow<WM>::bytes, RB = TileRow<WN>::bytes;
+    constexpr int STAGE = kBigBK * (RA + RB);
+    constexpr int ACH = RA / 16, BCH = RB / 32;             // slots of a row: chunks of 8 columns of a, of 16 of the codes
+    constexpr int AP = kBigBK * ACH / 256, BP = kBigBK * BCH / 256;   // passes of the 256 threads over a stage
+    constexpr int AROWS = 256 / ACH, BROWS = 256 / BCH;     // rows a pass
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tiles = g.tiles_m * g.tiles_n, total = tiles * g.splits;
+    // consecutive units on one XCD (workgroups go round the eight of them): the tiles of a row range share its L2
+    const int per = (total + 7) / 8, unit = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
+    if (blockIdx.x / 8 >= per || unit >= total) return;
+    const int split = unit / tiles, tile = unit % tiles;
+    const int m0 = (tile / g.tiles_n) * TMB, tn = tile % g.tiles_n, n0 = tn * TNB;
+    const int64_t k0 = (int64_t)split * g.rows_split;
+    const int64_t k1 = k0 + g.rows_split < g.rows ? k0 + g.rows_split : g.rows;
+    const int stages = (int)((k1 - k0 + kBigBK - 1) / kBigBK);
+
+    const int ach = tid % ACH, arow = tid / ACH, bch = tid % BCH, brow = tid / BCH;
+    int ma = m0 + 8 * ach, nb = n0 + 16 * bch;
+    ma = ma + 8 <= g.M ? ma : g.M - 8;
+    nb = nb + 16 <= g.npad ? nb : g.npad - 16;
+    u32x4a ra[AP], rb[BP];
+    uint2 rm[AP];
+    uint32_t rs[BP];
+    // rows of a stage: all there, or the last one's remainder, whose other rows repeat the last and are zeroed on the way in
+    auto load_a = [&](int i, int stage) {
+        const int64_t base = k0 + (int64_t)stage * kBigBK;
+        const int left = (int)(k1 - base < kBigBK ? k1 - base : kBigBK) - 1;
+        int r = arow + AROWS * i;
+        r = r < left ? r : left;
+        const u32x4u2 v = *reinterpret_cast<const u32x4u2*>(reinterpret_cast<const char*>(g.a + base * g.lda) + (uint32_t)((r * (int)g.lda + ma) * 2));
+        ra[i] = u32x4a{v[0], v[1], v[2], v[3]};
+        if constexpr (MASK) {
+            typedef uint32_t u32x2u1 __attribute__((ext_vector_type(2), aligned(1)));
+            const u32x2u1 c = *reinterpret_cast<const u32x2u1*>(g.mask + base * g.ld_mask + (uint32_t)(r * (int)g.ld_mask + ma));
+            rm[i] = make_uint2(c[0], c[1]);
+        }
+    };
+    auto load_b = [&](int i, int stage) {
+        const int64_t base = k0 + (int64_t)stage * kBigBK;
+        const int left = (int)(k1 - base < kBigBK ? k1 - base : kBigBK) - 1;
+        int r = brow + BROWS * i;
+        r = r < left ? r : left;
+        rb[i] = *reinterpret_cast<const u32x4a*>(g.codes + base * g.ld_codes + (uint32_t)(r * (int)g.ld_codes + nb));
+        rs[i] = (g.scales + base * g.ld_scales)[(uint32_t)(r * (int)g.ld_scales + nb / equss::kCkptBlock)];
+    };
+    float bsum[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) bsum[j] = 0.f;
+    auto store_a = [&](int i, int stage, char* sb) {
+        const int r = arow + AROWS * i;
+        u32x4a v = ra[i];
+        if constexpr (MASK) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t w = (j & 2 ? rm[i].y : rm[i].x) >> (16 * (j & 1));
+                v[j] &= ((int8_t)w > 0 ? 0xffffu : 0u) | ((int8_t)(w >> 8) > 0 ? 0xffff0000u : 0u);
+            }
+        }
+        if (k0 + (int64_t)stage * kBigBK + r >= k1) v = u32x4a{0, 0, 0, 0};
+        // the bias: every tile of a row of tiles adds up its share of the stages
+        if (g.bias && stage % g.tiles_n == tn) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                bsum[2 * j] += equss::bits_as<float>(v[j] << 16);
+                bsum[2 * j + 1] += equss::bits_as<float>(v[j] & 0xffff0000u);
+            }
+        }
+        *reinterpret_cast<u32x4a*>(sb + r * RA + ((ach ^ (4 * (r & 3))) * 16)) = v;
+    };
+    auto store_b = [&](int i, int stage, char* sb) {
+        const int r = brow + BROWS * i;
+        uint32_t sc = rs[i];
+        u32x4a c = rb[i];
+        if (k0 + (int64_t)stage * kBigBK + r >= k1) { sc = 0; c = u32x4a{0, 0, 0, 0}; }
+        const float s = equss::ckpt_scale(sc);
+        char* row = sb + kBigBK * RA + r * RB;
+        *reinterpret_cast<u32x4a*>(row + (((2 * bch) ^ (4 * (r & 3))) * 16)) = to_bf16x8<E4M3>(c[0], c[1], s);
+        *reinterpret_cast<u32x4a*>(row + (((2 * bch + 1) ^ (4 * (r & 3))) * 16)) = to_bf16x8<E4M3>(c[2], c[3], s);
+    };
+
+    const int wm = wave >> 1, wn = wave & 1;
+    const int q = (lane >> 2) & 3, pp = lane & 3, hg = (lane >> 4) & 1, kb = lane >> 5;
+    auto frag_at = [&](int c0, int row_bytes) {
+        const int chunk = c0 / 8 + 2 * hg + (pp >> 1);
+        return (8 * kb + q) * row_bytes + ((chunk ^ (4 * q)) * 16) + (pp & 1) * 8;
+    };
+    typedef __attribute__((address_space(3))) i16x4* lds_p;
+    auto frag = [&](const char* at, int row_bytes) {
+        const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(at));
+        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(at + 4 * row_bytes));
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    int a_at[WM], b_at[WN];
+#pragma unroll
+    for (int t = 0; t < WM; ++t) a_at[t] = frag_at((wm * WM + t) * 32, RA);
+#pragma unroll
+    for (int t = 0; t < WN; ++t) b_at[t] = kBigBK * RA + frag_at((wn * WN + t) * 32, RB);
+    f32x16 acc[WM][WN];
+#pragma unroll
+    for (int i = 0; i < WM; ++i)
+#pragma unroll
+        for (int j = 0; j < WN; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+
+    if (stages > 0) {
+#pragma unroll
+        for (int i = 0; i < AP; ++i) load_a(i, 0);
+#pragma unroll
+        for (int i = 0; i < BP; ++i) load_b(i, 0);
+#pragma unroll
+        for (int i = 0; i < AP; ++i) store_a(i, 0, smem);
+#pragma unroll
+        for (int i = 0; i < BP; ++i) store_b(i, 0, smem);
+        const int s1 = stages > 1 ? 1 : 0;
+#pragma unroll
+        for (int i = 0; i < AP; ++i) load_a(i, s1);
+#pragma unroll
+        for (int i = 0; i < BP; ++i) load_b(i, s1);
+    }
+    __syncthreads();
+    for (int stage = 0; stage < stages; ++stage) {
+        const char* cur = smem + (stage & 1) * STAGE;
+        char* nxt = smem + ((stage & 1) ^ 1) * STAGE;
+        const int s2 = stage + 2 < stages ? stage + 2 : stages - 1;
+        const bool more = stage + 1 < stages;
+#pragma unroll
+        for (int ks = 0; ks < kBigBK / 16; ++ks) {
+            bf16x8 af[WM], bf[WN];
+#pragma unroll
+            for (int t = 0; t < WM; ++t) af[t] = frag(cur + ks * 16 * RA + a_at[t], RA);
+#pragma unroll
+            for (int t = 0; t < WN; ++t) bf[t] = frag(cur + ks * 16 * RB + b_at[t], RB);
+            if (more) {
+#pragma unroll
+                for (int i = ks * AP / 4; i < (ks + 1) * AP / 4; ++i) { store_a(i, stage + 1, nxt); load_a(i, s2); }
+#pragma unroll
+                for (int i = ks * BP / 4; i < (ks + 1) * BP / 4; ++i) { store_b(i, stage + 1, nxt); load_b(i, s2); }
+            }
+#pragma unroll
+            for (int i = 0; i < WM; ++i)
+#pragma unroll
+                for (int j = 0; j < WN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[i], bf[j], acc[i][j], 0, 0, 0);
+        }
+        __syncthreads();
+    }
+
+    float* c = g.c + split * g.split_c;
+#pragma unroll
+    for (int i = 0; i < WM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int chunk = m0 + (wm * WM + i) * 32 + 8 * (r >> 2);
+            if (chunk < g.M) {
+                const int m = (chunk + 8 <= g.M ? chunk : g.M - 8) + 4 * kb + (r & 3);
+#pragma unroll
+                for (int j = 0; j < WN; ++j) {
+                    const int n = n0 + (wn * WN + j) * 32 + (lane & 31);
+                    if (n < g.N) c[m * g.ldc + n] = acc[i][j][r];
+                }
+            }
+        }
+    if (g.bias) {
+        float* part = reinterpret_cast<float*>(smem);      // (every reader of the tiles is behind the loop's last barrier)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) part[arow * (8 * ACH) + 8 * ach + j] = bsum[j];
+        __syncthreads();
+        const int chunk = m0 + tid / 8 * 8;
+        if (tid < TMB && chunk < g.M) {
+            float s = 0.f;
+            for (int r = 0; r < AROWS; ++r) s += part[r * (8 * ACH) + tid];
+            g.bias[(split * g.tiles_n + tn) * g.split_bias + (chunk + 8 <= g.M ? chunk : g.M - 8) + tid % 8] = s;
+        }
+    }
+}
+
 // C = sum of the partial products, in the order of the splits; then the bias
 __global__ __launch_bounds__(256) void gemm_tn_join_kernel(const float* __restrict__ part, int64_t split_c, float* __restrict__ c,
                                                           int64_t ldc, const float* __restrict__ bpart, int64_t split_bias,
-                                                          float* __restrict__ bias, int splits, int M, int N) {
+                                                          float* __restrict__ bias, int splits, int bias_splits, int M, int N, int bias_len) {
     const int64_t cells = (int64_t)M * N;
-    const int64_t total = cells + (bias ? M : 0);
+    const int64_t total = cells + (bias ? bias_len : 0);
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         const bool main = i < cells;
         const float* p = main ? part + i : bpart + (i - cells);
         const int64_t step = main ? split_c : split_bias;
+        const int n = main ? splits : bias_splits;
         float s = 0.f;
-        for (int k = 0; k < splits; ++k) s += p[k * step];
+        int k = 0;
+        for (; k + 8 <= n; k += 8) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = p[(k + j) * step];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s += v[j];
+        }
+        for (; k < n; ++k) s += p[k * step];
         if (main) c[(i / N) * ldc + i % N] = s;
         else bias[i - cells] = s;
     }
 }
 
-struct Plan { int tiles_m, tiles_n, splits; int64_t rows_split; };
+struct Plan { bool big; int tiles_m, tiles_n, splits, bias_splits; int64_t rows_split; };
 
 Plan plan(int64_t rows, int M, int N) {
     Plan p;
-    p.tiles_m = (M + TM - 1) / TM;
-    p.tiles_n = (N + TN - 1) / TN;
+    p.big = M > 128 && N > 128;
+    const int tm = p.big ? 256 : TM, tn = p.big ? 256 : TN, bk = p.big ? kBigBK : BK;
+    p.tiles_m = (M + tm - 1) / tm;
+    p.tiles_n = (N + tn - 1) / tn;
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-    int64_t splits = (512 + tiles - 1) / tiles;
-    const int64_t most = (rows + 4 * BK - 1) / (4 * BK);          // at least four steps a workgroup
+    int64_t splits = p.big ? 256 / tiles : (512 + tiles - 1) / tiles;
+    const int64_t most = (rows + 4 * bk - 1) / (4 * bk);          // at least four steps a workgroup
     if (splits > most) splits = most;
     if (splits < 1) splits = 1;
-    p.rows_split = ((rows + splits - 1) / splits + BK - 1) / BK * BK;
-    if (p.rows_split < BK) p.rows_split = BK;
+    p.rows_split = ((rows + splits - 1) / splits + bk - 1) / bk * bk;
+    if (p.rows_split < bk) p.rows_split = bk;
     p.splits = (int)((rows + p.rows_split - 1) / p.rows_split);
     if (p.splits < 1) p.splits = 1;
+    p.bias_splits = p.big ? p.splits * p.tiles_n : p.splits;
     return p;
 }
 
-size_t workspace(const Plan& p, int M, int N) { return p.splits == 1 ? 0 : (size_t)p.splits * ((size_t)M * N + M) * sizeof(float); }
+// partial products and, behind them, partial bias sums; nothing where one row range and one tile across write the results
+size_t workspace(const Plan& p, int M, int N) {
+    const size_t c = p.splits == 1 ? 0 : (size_t)p.splits * M * N, b = p.bias_splits == 1 ? 0 : (size_t)p.bias_splits * M;
+    return (c + b) * sizeof(float);
+}
 
 }  // namespace
 
@@ -254,31 +468,51 @@ extern "C" int equss_gemm_tn_ckpt(const void* a, int64_t lda, const void* codes,
     const int64_t blocks = (int64_t)p.tiles_m * p.tiles_n * p.splits;
     if (blocks > 0x7fffffff || (p.rows_split + BK - 1) / BK > 0x7fffffff)
         return equss::fail(EQUSS_E_UNSUPPORTED, "equss_gemm_tn_ckpt: %lld rows, M=%d N=%d", (long long)rows, M, N);
+    // (offsets within a stage of 64 rows are 32 bits)
+    if (rows > 0 && (lda > (1 << 23) || ld_codes > (1 << 23) || ld_relu > (1 << 23)))
+        return equss::fail(EQUSS_E_UNSUPPORTED, "equss_gemm_tn_ckpt: a leading dimension exceeds %d", 1 << 23);
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     g.a = reinterpret_cast<const u16*>(a); g.lda = lda;
     g.codes = reinterpret_cast<const uint8_t*>(codes); g.ld_codes = ld_codes;
     g.scales = reinterpret_cast<const uint8_t*>(scales); g.ld_scales = ld_scales;
     g.mask = reinterpret_cast<const uint8_t*>(relu_codes); g.ld_mask = ld_relu;
-    g.rows = rows; g.rows_split = p.rows_split; g.M = M; g.N = N; g.tiles_m = p.tiles_m; g.tiles_n = p.tiles_n;
+    g.rows = rows; g.rows_split = p.rows_split; g.M = M; g.N = N; g.tiles_m = p.tiles_m; g.tiles_n = p.tiles_n; g.splits = p.splits;
     float* part = reinterpret_cast<float*>(workspace_ptr);
-    float* bpart = part + (size_t)p.splits * M * N;
-    const bool direct = p.splits == 1;
+    float* bpart = part + (p.splits == 1 ? 0 : (size_t)p.splits * M * N);
+    const bool direct = p.splits == 1, bias_direct = p.bias_splits == 1;
     g.c = direct ? C : part; g.ldc = direct ? ldc : N; g.split_c = direct ? 0 : (int64_t)M * N;
-    g.bias = bias ? (direct ? bias : bpart) : nullptr; g.split_bias = direct ? 0 : M;
-    const dim3 grid((unsigned)blocks), block(kTnThreads);
-    if (fmt == EQUSS_CKPT_E4M3) {
-        if (relu_codes) hipLaunchKernelGGL((gemm_tn_ckpt_kernel<true, true>), grid, block, 0, s, g);
-        else hipLaunchKernelGGL((gemm_tn_ckpt_kernel<true, false>), grid, block, 0, s, g);
+    g.bias = bias ? (bias_direct ? bias : bpart) : nullptr; g.split_bias = M;
+    const bool e = fmt == EQUSS_CKPT_E4M3;
+    if (p.big) {
+        const int lds = 2 * kBigBK * 1024;
+        const dim3 grid((unsigned)((blocks + 7) / 8 * 8));
+#define EQUSS_TN_BIG(E, K)                                                                                                     \
+    do {                                                                                                                       \
+        if (!equss::lds_opt_in(reinterpret_cast<const void*>(&gemm_tn_ckpt_big_kernel<E, K, 4, 4>), lds))                      \
+            return equss::fail(EQUSS_E_UNSUPPORTED, "equss_gemm_tn_ckpt: %d bytes of LDS", lds);                               \
+        hipLaunchKernelGGL((gemm_tn_ckpt_big_kernel<E, K, 4, 4>), grid, dim3(256), lds, s, g);                                 \
+    } while (0)
+        if (e) { if (relu_codes) EQUSS_TN_BIG(true, true); else EQUSS_TN_BIG(true, false); }
+        else { if (relu_codes) EQUSS_TN_BIG(false, true); else EQUSS_TN_BIG(false, false); }
+#undef EQUSS_TN_BIG
     } else {
-        if (relu_codes) hipLaunchKernelGGL((gemm_tn_ckpt_kernel<false, true>), grid, block, 0, s, g);
-        else hipLaunchKernelGGL((gemm_tn_ckpt_kernel<false, false>), grid, block, 0, s, g);
+        const dim3 grid((unsigned)blocks), block(kTnThreads);
+        if (e) {
+            if (relu_codes) hipLaunchKernelGGL((gemm_tn_ckpt_kernel<true, true>), grid, block, 0, s, g);
+            else hipLaunchKernelGGL((gemm_tn_ckpt_kernel<true, false>), grid, block, 0, s, g);
+        } else {
+            if (relu_codes) hipLaunchKernelGGL((gemm_tn_ckpt_kernel<false, true>), grid, block, 0, s, g);
+            else hipLaunchKernelGGL((gemm_tn_ckpt_kernel<false, false>), grid, block, 0, s, g);
+        }
     }
     const int rc = equss::check_launch("gemm_tn_ckpt_kernel");
-    if (rc != EQUSS_OK || direct) return rc;
-    const int64_t total = (int64_t)M * N + (bias ? M : 0);
+    const bool join_bias = bias && !bias_direct;
+    if (rc != EQUSS_OK || (direct && !join_bias)) return rc;
+    // (with one row range the products are in place and only the bias is left)
+    const int64_t total = (direct ? 0 : (int64_t)M * N) + (join_bias ? M : 0);
     int64_t gx = (total + 255) / 256;
     if (gx > 4096) gx = 4096;
-    hipLaunchKernelGGL(gemm_tn_join_kernel, dim3((unsigned)gx), dim3(256), 0, s, part, (int64_t)M * N, C, ldc, bpart, (int64_t)M, bias,
-                       p.splits, M, N);
+    hipLaunchKernelGGL(gemm_tn_join_kernel, dim3((unsigned)gx), dim3(256), 0, s, part, (int64_t)M * N, C, ldc, bpart, (int64_t)M,
+                       join_bias ? bias : nullptr, p.splits, p.bias_splits, direct ? 0 : M, direct ? 1 : N, M);
     return equss::check_launch("gemm_tn_join_kernel");
 }
