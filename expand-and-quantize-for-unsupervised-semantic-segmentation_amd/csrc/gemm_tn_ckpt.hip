@@ -187,29 +187,40 @@ __global__ __launch_bounds__(kTnThreads, 2) void gemm_tn_ckpt_kernel(const Args 
     }
 }
 
-// ---- the large tile: 4 waves, WM x WN MFMA tiles of 32 x 32 each, i.e. 64 WM x 64 WN of C; 64 rows a stage, two stages in LDS.
-// A wave's accumulators take up to 256 registers, so one wave a SIMD; what hides its latencies is its own pipeline: while it
-// multiplies stage s out of LDS, the registers hold stage s + 1 (requested a whole stage earlier), which goes through the
-// conversion into the other half of LDS a quarter at a time, each quarter's registers being refilled at once from stage s + 2.
-// Columns past M: the last chunk of 8 columns is read at M - 8, so that every load is whole and inside; the chunk's columns
-// then overlap the chunk before, both give the same sums, and both are written.  Columns past N lie in the checkpoint's
-// padding or are read from its last block; their sums are dropped.
-constexpr int kBigBK = 64;
+// ---- the large tile: 4 waves of WM x WN MFMA tiles of 32 x 32, i.e. 64 WM x 64 WN of C; 32 rows a stage, three stages in LDS.
+// A wave's accumulators take up to 256 registers, so there is one wave a SIMD, and what hides its latencies is its own pipeline.
+// While a stage's fragments are multiplied,
+//   the fragments of the next half stage are read (the next stage's first half too: its writes are a barrier back),
+//   the stage after the next goes from registers through the conversion into the third slot of LDS, and
+//   each of those registers is requested again from two stages further on (there are two sets of them: one stage of 32 rows
+//   takes half a microsecond, less than a load from memory does under load),
+// without a branch in between, so that the scheduler can put all of it between the MFMAs.
+// Columns past M: the last chunk of 8 columns is read at M - 8, so that every load is whole and inside; its columns then
+// overlap the chunk before, both give the same sums, and both are written.  Columns past N lie in the checkpoint's padding or
+// are read from its last block; their sums are dropped.
+constexpr int kBigBK = 32, kSlots = 3;
 
 template <int T64> struct TileRow { static constexpr int bytes = T64 == 2 ? 256 : 512; };   // (192 columns in rows of 512: the swizzle's xor needs them)
 
 template <bool E4M3>
 __device__ __forceinline__ u32x4a to_bf16x8(uint32_t c0, uint32_t c1, float s) {
-    const f32x4 lo = equss::ckpt_decode4<E4M3>(c0), hi = equss::ckpt_decode4<E4M3>(c1);
-    return u32x4a{equss::pack_bf16(lo[0] * s, lo[1] * s), equss::pack_bf16(lo[2] * s, lo[3] * s),
-                  equss::pack_bf16(hi[0] * s, hi[1] * s), equss::pack_bf16(hi[2] * s, hi[3] * s)};
+    if constexpr (E4M3) {
+        typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+        const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c0, s, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c0, s, true);
+        const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c1, s, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c1, s, true);
+        return u32x4a{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, d)};
+    } else {
+        const f32x4 lo = equss::ckpt_decode4<false>(c0), hi = equss::ckpt_decode4<false>(c1);
+        return u32x4a{equss::pack_bf16(lo[0] * s, lo[1] * s), equss::pack_bf16(lo[2] * s, lo[3] * s),
+                      equss::pack_bf16(hi[0] * s, hi[1] * s), equss::pack_bf16(hi[2] * s, hi[3] * s)};
+    }
 }
 
 template <bool E4M3, bool MASK, int WM, int WN>
 __global__ __launch_bounds__(256, 1) void gemm_tn_ckpt_big_kernel(const Args g) {
     constexpr int TMB = 64 * WM, TNB = 64 * WN, RA = TileRow<WM>::bytes, RB = TileRow<WN>::bytes;
-    constexpr int STAGE = kBigBK * (RA + RB);
-    constexpr int ACH = RA / 16, BCH = RB / 32;             // slots of a row: chunks of 8 columns of a, of 16 of the codes
+    constexpr int SLOT = kBigBK * (RA + RB);
+    constexpr int ACH = RA / 16, BCH = RB / 32;             // a row's chunks of 8 columns of a, of 16 codes
     constexpr int AP = kBigBK * ACH / 256, BP = kBigBK * BCH / 256;   // passes of the 256 threads over a stage
     constexpr int AROWS = 256 / ACH, BROWS = 256 / BCH;     // rows a pass
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -218,71 +229,91 @@ __global__ __launch_bounds__(256, 1) void gemm_tn_ckpt_big_kernel(const Args g) 
     const int tiles = g.tiles_m * g.tiles_n, total = tiles * g.splits;
     // consecutive units on one XCD (workgroups go round the eight of them): the tiles of a row range share its L2
     const int per = (total + 7) / 8, unit = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
-    if (blockIdx.x / 8 >= per || unit >= total) return;
+    if ((int)(blockIdx.x / 8) >= per || unit >= total) return;
     const int split = unit / tiles, tile = unit % tiles;
     const int m0 = (tile / g.tiles_n) * TMB, tn = tile % g.tiles_n, n0 = tn * TNB;
     const int64_t k0 = (int64_t)split * g.rows_split;
     const int64_t k1 = k0 + g.rows_split < g.rows ? k0 + g.rows_split : g.rows;
-    const int stages = (int)((k1 - k0 + kBigBK - 1) / kBigBK);
+    const int rows = (int)(k1 - k0);
+    const int stages = (rows + kBigBK - 1) / kBigBK, whole = rows / kBigBK;
 
+    // ---- staging.  Addresses are a uniform part (stage and pass) and a lane's 32-bit offset within a stage.
     const int ach = tid % ACH, arow = tid / ACH, bch = tid % BCH, brow = tid / BCH;
     int ma = m0 + 8 * ach, nb = n0 + 16 * bch;
     ma = ma + 8 <= g.M ? ma : g.M - 8;
     nb = nb + 16 <= g.npad ? nb : g.npad - 16;
-    u32x4a ra[AP], rb[BP];
-    uint2 rm[AP];
-    uint32_t rs[BP];
-    // rows of a stage: all there, or the last one's remainder, whose other rows repeat the last and are zeroed on the way in
-    auto load_a = [&](int i, int stage) {
-        const int64_t base = k0 + (int64_t)stage * kBigBK;
-        const int left = (int)(k1 - base < kBigBK ? k1 - base : kBigBK) - 1;
-        int r = arow + AROWS * i;
-        r = r < left ? r : left;
-        const u32x4u2 v = *reinterpret_cast<const u32x4u2*>(reinterpret_cast<const char*>(g.a + base * g.lda) + (uint32_t)((r * (int)g.lda + ma) * 2));
-        ra[i] = u32x4a{v[0], v[1], v[2], v[3]};
+    const int lda = (int)g.lda, ldc = (int)g.ld_codes, lds = (int)g.ld_scales, ldm = (int)g.ld_mask;
+    const uint32_t va = (uint32_t)((arow * lda + ma) * 2), vm = (uint32_t)(arow * ldm + ma);
+    const uint32_t vb = (uint32_t)(brow * ldc + nb), vs = (uint32_t)(brow * lds + nb / equss::kCkptBlock);
+    u32x4a ra[2][AP], rb[2][BP];
+    uint2 rm[2][AP];
+    uint32_t rs[2][BP];
+    typedef uint32_t u32x2u1 __attribute__((ext_vector_type(2), aligned(1)));
+    // LAST: the stage's rows may end before its 32: the others repeat the last one (and are zeroed on their way into LDS)
+    auto load_a = [&](auto last_c, int set, int i, int stage) __attribute__((always_inline)) {
+        constexpr bool LAST = decltype(last_c)::value;
+        const int64_t row = k0 + (int64_t)stage * kBigBK + (LAST ? 0 : AROWS * i);
+        uint32_t oa = va, om = vm;
+        if constexpr (LAST) {
+            const int left = rows - stage * kBigBK - 1, r = arow + AROWS * i < left ? arow + AROWS * i : left;
+            oa = (uint32_t)((r * lda + ma) * 2);
+            om = (uint32_t)(r * ldm + ma);
+        }
+        const u32x4u2 v = *reinterpret_cast<const u32x4u2*>(reinterpret_cast<const char*>(g.a + row * g.lda) + oa);
+        ra[set][i] = u32x4a{v[0], v[1], v[2], v[3]};
         if constexpr (MASK) {
-            typedef uint32_t u32x2u1 __attribute__((ext_vector_type(2), aligned(1)));
-            const u32x2u1 c = *reinterpret_cast<const u32x2u1*>(g.mask + base * g.ld_mask + (uint32_t)(r * (int)g.ld_mask + ma));
-            rm[i] = make_uint2(c[0], c[1]);
+            const u32x2u1 c = *reinterpret_cast<const u32x2u1*>(g.mask + row * g.ld_mask + om);
+            rm[set][i] = make_uint2(c[0], c[1]);
         }
     };
-    auto load_b = [&](int i, int stage) {
-        const int64_t base = k0 + (int64_t)stage * kBigBK;
-        const int left = (int)(k1 - base < kBigBK ? k1 - base : kBigBK) - 1;
-        int r = brow + BROWS * i;
-        r = r < left ? r : left;
-        rb[i] = *reinterpret_cast<const u32x4a*>(g.codes + base * g.ld_codes + (uint32_t)(r * (int)g.ld_codes + nb));
-        rs[i] = (g.scales + base * g.ld_scales)[(uint32_t)(r * (int)g.ld_scales + nb / equss::kCkptBlock)];
+    auto load_b = [&](auto last_c, int set, int i, int stage) __attribute__((always_inline)) {
+        constexpr bool LAST = decltype(last_c)::value;
+        const int64_t row = k0 + (int64_t)stage * kBigBK + (LAST ? 0 : BROWS * i);
+        uint32_t ob = vb, os = vs;
+        if constexpr (LAST) {
+            const int left = rows - stage * kBigBK - 1, r = brow + BROWS * i < left ? brow + BROWS * i : left;
+            ob = (uint32_t)(r * ldc + nb);
+            os = (uint32_t)(r * lds + nb / equss::kCkptBlock);
+        }
+        rb[set][i] = *reinterpret_cast<const u32x4a*>(g.codes + row * g.ld_codes + ob);
+        rs[set][i] = (g.scales + row * g.ld_scales)[os];
     };
     float bsum[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) bsum[j] = 0.f;
-    auto store_a = [&](int i, int stage, char* sb) {
+    // the bias: every tile of a row of tiles adds up its share of the stages, [bias0, bias1); even ones, as the loop goes by two
+    const int bias0 = g.bias ? (int)((int64_t)stages * tn / g.tiles_n) & ~1 : 0;
+    const int bias1 = !g.bias ? 0 : tn + 1 == g.tiles_n ? stages : (int)((int64_t)stages * (tn + 1) / g.tiles_n) & ~1;
+    auto store_a = [&](auto last_c, auto bias_c, int set, int i, int stage, char* sb) __attribute__((always_inline)) {
         const int r = arow + AROWS * i;
-        u32x4a v = ra[i];
+        u32x4a v = ra[set][i];
         if constexpr (MASK) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const uint32_t w = (j & 2 ? rm[i].y : rm[i].x) >> (16 * (j & 1));
+                const uint32_t w = (j & 2 ? rm[set][i].y : rm[set][i].x) >> (16 * (j & 1));
                 v[j] &= ((int8_t)w > 0 ? 0xffffu : 0u) | ((int8_t)(w >> 8) > 0 ? 0xffff0000u : 0u);
             }
         }
-        if (k0 + (int64_t)stage * kBigBK + r >= k1) v = u32x4a{0, 0, 0, 0};
-        // the bias: every tile of a row of tiles adds up its share of the stages
-        if (g.bias && stage % g.tiles_n == tn) {
+        if constexpr (decltype(last_c)::value) {
+            if (stage * kBigBK + r >= rows) v = u32x4a{0, 0, 0, 0};
+        }
+        if constexpr (decltype(bias_c)::value) {
+            const uint32_t mine = !decltype(last_c)::value || (stage >= bias0 && stage < bias1) ? 0xffffffffu : 0u;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                bsum[2 * j] += equss::bits_as<float>(v[j] << 16);
-                bsum[2 * j + 1] += equss::bits_as<float>(v[j] & 0xffff0000u);
+                bsum[2 * j] += equss::bits_as<float>((v[j] & mine) << 16);
+                bsum[2 * j + 1] += equss::bits_as<float>(v[j] & mine & 0xffff0000u);
             }
         }
         *reinterpret_cast<u32x4a*>(sb + r * RA + ((ach ^ (4 * (r & 3))) * 16)) = v;
     };
-    auto store_b = [&](int i, int stage, char* sb) {
+    auto store_b = [&](auto last_c, int set, int i, int stage, char* sb) __attribute__((always_inline)) {
         const int r = brow + BROWS * i;
-        uint32_t sc = rs[i];
-        u32x4a c = rb[i];
-        if (k0 + (int64_t)stage * kBigBK + r >= k1) { sc = 0; c = u32x4a{0, 0, 0, 0}; }
+        uint32_t sc = rs[set][i];
+        u32x4a c = rb[set][i];
+        if constexpr (decltype(last_c)::value) {
+            if (stage * kBigBK + r >= rows) { sc = 0; c = u32x4a{0, 0, 0, 0}; }
+        }
         const float s = equss::ckpt_scale(sc);
         char* row = sb + kBigBK * RA + r * RB;
         *reinterpret_cast<u32x4a*>(row + (((2 * bch) ^ (4 * (r & 3))) * 16)) = to_bf16x8<E4M3>(c[0], c[1], s);
@@ -291,12 +322,12 @@ __global__ __launch_bounds__(256, 1) void gemm_tn_ckpt_big_kernel(const Args g) 
 
     const int wm = wave >> 1, wn = wave & 1;
     const int q = (lane >> 2) & 3, pp = lane & 3, hg = (lane >> 4) & 1, kb = lane >> 5;
-    auto frag_at = [&](int c0, int row_bytes) {
+    auto frag_at = [&](int c0, int row_bytes) __attribute__((always_inline)) {
         const int chunk = c0 / 8 + 2 * hg + (pp >> 1);
         return (8 * kb + q) * row_bytes + ((chunk ^ (4 * q)) * 16) + (pp & 1) * 8;
     };
     typedef __attribute__((address_space(3))) i16x4* lds_p;
-    auto frag = [&](const char* at, int row_bytes) {
+    auto frag = [&](const char* at, int row_bytes) __attribute__((always_inline)) {
         const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(at));
         const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(at + 4 * row_bytes));
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -306,6 +337,13 @@ __global__ __launch_bounds__(256, 1) void gemm_tn_ckpt_big_kernel(const Args g) 
     for (int t = 0; t < WM; ++t) a_at[t] = frag_at((wm * WM + t) * 32, RA);
 #pragma unroll
     for (int t = 0; t < WN; ++t) b_at[t] = kBigBK * RA + frag_at((wn * WN + t) * 32, RB);
+    bf16x8 af[2][WM], bf[2][WN];
+    auto read = [&](int set, const char* slot, int ks) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < WM; ++t) af[set][t] = frag(slot + ks * 16 * RA + a_at[t], RA);
+#pragma unroll
+        for (int t = 0; t < WN; ++t) bf[set][t] = frag(slot + ks * 16 * RB + b_at[t], RB);
+    };
     f32x16 acc[WM][WN];
 #pragma unroll
     for (int i = 0; i < WM; ++i)
@@ -313,47 +351,95 @@ __global__ __launch_bounds__(256, 1) void gemm_tn_ckpt_big_kernel(const Args g) 
         for (int j = 0; j < WN; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-
-    if (stages > 0) {
+    auto multiply = [&](int set) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < AP; ++i) load_a(i, 0);
+        for (int i = 0; i < WM; ++i)
 #pragma unroll
-        for (int i = 0; i < BP; ++i) load_b(i, 0);
+            for (int j = 0; j < WN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[set][i], bf[set][j], acc[i][j], 0, 0, 0);
+    };
+    using No = std::false_type;
+    using Yes = std::true_type;
+    auto fetch = [&](int set, int stage) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < AP; ++i) store_a(i, 0, smem);
+        for (int i = 0; i < AP; ++i) load_a(Yes(), set, i, stage);
 #pragma unroll
-        for (int i = 0; i < BP; ++i) store_b(i, 0, smem);
-        const int s1 = stages > 1 ? 1 : 0;
+        for (int i = 0; i < BP; ++i) load_b(Yes(), set, i, stage);
+    };
+    auto put = [&](int set, int stage, char* slot) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < AP; ++i) load_a(i, s1);
+        for (int i = 0; i < AP; ++i) store_a(Yes(), Yes(), set, i, stage, slot);
 #pragma unroll
-        for (int i = 0; i < BP; ++i) load_b(i, s1);
-    }
-    __syncthreads();
-    for (int stage = 0; stage < stages; ++stage) {
-        const char* cur = smem + (stage & 1) * STAGE;
-        char* nxt = smem + ((stage & 1) ^ 1) * STAGE;
-        const int s2 = stage + 2 < stages ? stage + 2 : stages - 1;
-        const bool more = stage + 1 < stages;
+        for (int i = 0; i < BP; ++i) store_b(Yes(), set, i, stage, slot);
+    };
+    // one stage: multiply `stage`, read ahead, store stage + 2 and request stage + 4 (which are there and whole)
+    auto step = [&](auto bias_c, int set, int stage, const char* s0, const char* s1, char* s2) __attribute__((always_inline)) {
+        const No last_c;
 #pragma unroll
-        for (int ks = 0; ks < kBigBK / 16; ++ks) {
-            bf16x8 af[WM], bf[WN];
+        for (int ks = 0; ks < 2; ++ks) {
+            if (ks == 0) read(1, s0, 1);
+            else read(0, s1, 0);
 #pragma unroll
-            for (int t = 0; t < WM; ++t) af[t] = frag(cur + ks * 16 * RA + a_at[t], RA);
+            for (int i = ks * AP / 2; i < (ks + 1) * AP / 2; ++i) { store_a(last_c, bias_c, set, i, stage + 2, s2); load_a(last_c, set, i, stage + 4); }
 #pragma unroll
-            for (int t = 0; t < WN; ++t) bf[t] = frag(cur + ks * 16 * RB + b_at[t], RB);
-            if (more) {
+            for (int i = ks * BP / 2; i < (ks + 1) * BP / 2; ++i) { store_b(last_c, set, i, stage + 2, s2); load_b(last_c, set, i, stage + 4); }
+            multiply(ks);
+            // the order wanted: behind every MFMA two fragment reads (first half) or a store and its next request, and conversions
 #pragma unroll
-                for (int i = ks * AP / 4; i < (ks + 1) * AP / 4; ++i) { store_a(i, stage + 1, nxt); load_a(i, s2); }
-#pragma unroll
-                for (int i = ks * BP / 4; i < (ks + 1) * BP / 4; ++i) { store_b(i, stage + 1, nxt); load_b(i, s2); }
+            for (int i = 0; i < WM * WN; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);            // MFMA
+                if (i < WM + WN) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);   // LDS reads
+                __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);            // VALU
+                if (i >= WM * WN / 2) {
+                    __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);        // LDS write
+                    __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);        // global load
+                }
             }
-#pragma unroll
-            for (int i = 0; i < WM; ++i)
-#pragma unroll
-                for (int j = 0; j < WN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[i], bf[j], acc[i][j], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
         __syncthreads();
+    };
+
+    if (stages > 0) {
+        fetch(0, 0);
+        if (stages > 1) fetch(1, 1);
+        put(0, 0, smem);
+        if (stages > 2) fetch(0, 2);
+        if (stages > 1) put(1, 1, smem + SLOT);
+        if (stages > 3) fetch(1, 3);
+    }
+    __syncthreads();
+    if (stages > 0) read(0, smem, 0);
+    int stage = 0, slot = 0;
+    auto at = [&](int k) __attribute__((always_inline)) { return smem + (slot + k >= kSlots ? slot + k - kSlots : slot + k) * SLOT; };
+    auto next = [&]() __attribute__((always_inline)) {
+        ++stage;
+        slot = slot + 1 == kSlots ? 0 : slot + 1;
+    };
+    const int end = whole - 4;
+    auto run = [&](auto bias_c, int to) __attribute__((always_inline)) {
+        while (stage + 1 < to) {
+            step(bias_c, 0, stage, at(0), at(1), at(2));
+            next();
+            step(bias_c, 1, stage, at(0), at(1), at(2));
+            next();
+        }
+    };
+    run(No(), end < bias0 - 2 ? end : bias0 - 2);
+    run(Yes(), end < bias1 - 2 ? end : bias1 - 2);
+    run(No(), end);
+    auto last = [&](int set) __attribute__((always_inline)) {                              // the last few, one thing after the other
+        if (stage + 2 < stages) put(set, stage + 2, at(2));
+        if (stage + 4 < stages) fetch(set, stage + 4);
+        read(1, at(0), 1);
+        multiply(0);
+        if (stage + 1 < stages) read(0, at(1), 0);
+        multiply(1);
+        __syncthreads();
+        next();
+    };
+    while (stage < stages) {
+        last(0);
+        if (stage < stages) last(1);
     }
 
     float* c = g.c + split * g.split_c;
@@ -484,7 +570,7 @@ extern "C" int equss_gemm_tn_ckpt(const void* a, int64_t lda, const void* codes,
     g.bias = bias ? (bias_direct ? bias : bpart) : nullptr; g.split_bias = M;
     const bool e = fmt == EQUSS_CKPT_E4M3;
     if (p.big) {
-        const int lds = 2 * kBigBK * 1024;
+        const int lds = kSlots * kBigBK * 1024;
         const dim3 grid((unsigned)((blocks + 7) / 8 * 8));
 #define EQUSS_TN_BIG(E, K)                                                                                                     \
     do {                                                                                                                       \
