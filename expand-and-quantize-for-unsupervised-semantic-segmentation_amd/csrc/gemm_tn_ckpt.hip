@@ -31,7 +31,7 @@ struct Args {
     int64_t split_c;
     float* bias; int64_t split_bias;           // or null
     int64_t rows, rows_split;
-    int M, N, tiles_m, tiles_n, splits, npad, mpad;
+    int M, N, tiles_m, tiles_n, splits, bias_tiles, npad, mpad;
 };
 
 template <bool E4M3, bool MASK>
@@ -187,20 +187,22 @@ __global__ __launch_bounds__(kTnThreads, 2) void gemm_tn_ckpt_kernel(const Args 
     }
 }
 
-// ---- the large tile: 4 waves of WM x WN MFMA tiles of 32 x 32, i.e. 64 WM x 64 WN of C; 32 rows a stage, three stages in LDS.
-// A wave's accumulators take up to 256 registers, so there is one wave a SIMD, and what hides its latencies is its own pipeline.
-// While a stage's fragments are multiplied,
+// ---- square tiles of TILE = 256 (8 waves, two a SIMD, one workgroup a CU) or 128 (4 waves, two workgroups a CU) of C, in
+// 2 x TILE / 64 waves of TILE / 64 x 2 MFMA tiles of 32 x 32; 32 rows a stage, four stages in LDS.  While a stage's fragments are multiplied,
 //   the fragments of the next half stage are read (the next stage's first half too: its writes are a barrier back),
-//   the stage after the next goes from registers through the conversion into the third slot of LDS, and
+//   the stage after the next goes from registers through the conversion into its slot of LDS, and
 //   each of those registers is requested again from two stages further on (there are two sets of them: one stage of 32 rows
 //   takes half a microsecond, less than a load from memory does under load),
-// without a branch in between, so that the scheduler can put all of it between the MFMAs.
+// without a branch in between, so that the scheduler can put all of it between the MFMAs.  The loop goes by four stages, so that
+// slots and register sets are constants.  Loads past a workgroup's rows return zero (buffer addressing), codes and scales too:
+// the last stages need no care and the surplus ones of the last round multiply zeros.
+// Conversions, address arithmetic and the bias are what the matrix pipe waits for (counted: of 75 M issue cycles of the first
+// version with one wave a SIMD, the MFMAs took 39 M and other vector instructions 23 M, one after the other); hence two waves
+// a SIMD, constant LDS addresses and buffer loads.
 // Columns past M: the last chunk of 8 columns is read at M - 8, so that every load is whole and inside; its columns then
 // overlap the chunk before, both give the same sums, and both are written.  Columns past N lie in the checkpoint's padding or
 // are read from its last block; their sums are dropped.
-constexpr int kBigBK = 32, kSlots = 3;
-
-template <int T64> struct TileRow { static constexpr int bytes = T64 == 2 ? 256 : 512; };   // (192 columns in rows of 512: the swizzle's xor needs them)
+constexpr int kBigBK = 32, kSlots = 4;
 
 template <bool E4M3>
 __device__ __forceinline__ u32x4a to_bf16x8(uint32_t c0, uint32_t c1, float s) {
@@ -216,13 +218,22 @@ __device__ __forceinline__ u32x4a to_bf16x8(uint32_t c0, uint32_t c1, float s) {
     }
 }
 
-template <bool E4M3, bool MASK, int WM, int WN>
-__global__ __launch_bounds__(256, 1) void gemm_tn_ckpt_big_kernel(const Args g) {
-    constexpr int TMB = 64 * WM, TNB = 64 * WN, RA = TileRow<WM>::bytes, RB = TileRow<WN>::bytes;
-    constexpr int SLOT = kBigBK * (RA + RB);
-    constexpr int ACH = RA / 16, BCH = RB / 32;             // a row's chunks of 8 columns of a, of 16 codes
-    constexpr int AP = kBigBK * ACH / 256, BP = kBigBK * BCH / 256;   // passes of the 256 threads over a stage
-    constexpr int AROWS = 256 / ACH, BROWS = 256 / BCH;     // rows a pass
+// rows [row0, row0 + rows) of a matrix of `ld` bytes a row: loads past the end return zero
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* p, int64_t ld, int64_t row0, int rows) {
+    const uint64_t base = reinterpret_cast<uint64_t>(p) + (uint64_t)row0 * (uint64_t)ld;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)base), hi = __builtin_amdgcn_readfirstlane((uint32_t)(base >> 32));
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(((uint64_t)hi << 32) | lo), 0,
+                                             __builtin_amdgcn_readfirstlane((int)((int64_t)rows * ld)), 0x00020000);
+}
+
+template <bool E4M3, bool MASK, int TILE>
+__global__ __launch_bounds__(2 * TILE, 2) void gemm_tn_ckpt_tile_kernel(const Args g) {
+    constexpr int THREADS = 2 * TILE, WAVES_N = TILE / 64, WM = TILE / 64, WNW = 2;
+    constexpr int TMB = TILE, TNB = TILE, RA = 2 * TILE, RB = 2 * TILE, SLOT = kBigBK * (RA + RB);
+    constexpr int ACH = TILE / 8, BCH = TILE / 16;          // a row's chunks of 8 columns of a, of 16 codes
+    constexpr int AP = kBigBK * ACH / THREADS, BP = kBigBK * BCH / THREADS;   // passes of the threads over a stage: 2 and 1
+    constexpr int AROWS = THREADS / ACH, BROWS = THREADS / BCH;               // rows a pass
+    static_assert(AP == 2 && BP == 1, "one request of a a half stage, one of the codes a stage");
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -234,58 +245,56 @@ __global__ __launch_bounds__(256, 1) void gemm_tn_ckpt_big_kernel(const Args g) 
     const int m0 = (tile / g.tiles_n) * TMB, tn = tile % g.tiles_n, n0 = tn * TNB;
     const int64_t k0 = (int64_t)split * g.rows_split;
     const int64_t k1 = k0 + g.rows_split < g.rows ? k0 + g.rows_split : g.rows;
-    const int rows = (int)(k1 - k0);
-    const int stages = (rows + kBigBK - 1) / kBigBK, whole = rows / kBigBK;
+    const int rows = k1 > k0 ? (int)(k1 - k0) : 0;
+    const int stages = (rows + kBigBK - 1) / kBigBK;
 
-    // ---- staging.  Addresses are a uniform part (stage and pass) and a lane's 32-bit offset within a stage.
+    // ---- staging
     const int ach = tid % ACH, arow = tid / ACH, bch = tid % BCH, brow = tid / BCH;
     int ma = m0 + 8 * ach, nb = n0 + 16 * bch;
     ma = ma + 8 <= g.M ? ma : g.M - 8;
     nb = nb + 16 <= g.npad ? nb : g.npad - 16;
-    const int lda = (int)g.lda, ldc = (int)g.ld_codes, lds = (int)g.ld_scales, ldm = (int)g.ld_mask;
-    const uint32_t va = (uint32_t)((arow * lda + ma) * 2), vm = (uint32_t)(arow * ldm + ma);
-    const uint32_t vb = (uint32_t)(brow * ldc + nb), vs = (uint32_t)(brow * lds + nb / equss::kCkptBlock);
+    const __amdgpu_buffer_rsrc_t a_rs = rows_rsrc(g.a, g.lda * 2, k0, rows), b_rs = rows_rsrc(g.codes, g.ld_codes, k0, rows);
+    const __amdgpu_buffer_rsrc_t s_rs = rows_rsrc(g.scales, g.ld_scales, k0, rows), m_rs = rows_rsrc(g.mask, g.ld_mask, k0, MASK ? rows : 0);
+    // byte offsets of the next request of every pass
+    uint32_t va[AP], vm[AP], vb[BP], vs[BP];
+#pragma unroll
+    for (int i = 0; i < AP; ++i) {
+        va[i] = (uint32_t)(((arow + AROWS * i) * (int)g.lda + ma) * 2);
+        vm[i] = (uint32_t)((arow + AROWS * i) * (int)g.ld_mask + ma);
+    }
+#pragma unroll
+    for (int i = 0; i < BP; ++i) {
+        vb[i] = (uint32_t)((brow + BROWS * i) * (int)g.ld_codes + nb);
+        vs[i] = (uint32_t)((brow + BROWS * i) * (int)g.ld_scales + nb / equss::kCkptBlock);
+    }
+    const uint32_t da = (uint32_t)(kBigBK * 2 * (int)g.lda), dm = (uint32_t)(kBigBK * (int)g.ld_mask);
+    const uint32_t db = (uint32_t)(kBigBK * (int)g.ld_codes), ds = (uint32_t)(kBigBK * (int)g.ld_scales);
     u32x4a ra[2][AP], rb[2][BP];
     uint2 rm[2][AP];
     uint32_t rs[2][BP];
-    typedef uint32_t u32x2u1 __attribute__((ext_vector_type(2), aligned(1)));
-    // LAST: the stage's rows may end before its 32: the others repeat the last one (and are zeroed on their way into LDS)
-    auto load_a = [&](auto last_c, int set, int i, int stage) __attribute__((always_inline)) {
-        constexpr bool LAST = decltype(last_c)::value;
-        const int64_t row = k0 + (int64_t)stage * kBigBK + (LAST ? 0 : AROWS * i);
-        uint32_t oa = va, om = vm;
-        if constexpr (LAST) {
-            const int left = rows - stage * kBigBK - 1, r = arow + AROWS * i < left ? arow + AROWS * i : left;
-            oa = (uint32_t)((r * lda + ma) * 2);
-            om = (uint32_t)(r * ldm + ma);
-        }
-        const u32x4u2 v = *reinterpret_cast<const u32x4u2*>(reinterpret_cast<const char*>(g.a + row * g.lda) + oa);
-        ra[set][i] = u32x4a{v[0], v[1], v[2], v[3]};
+    auto load_a = [&](int set, int i) __attribute__((always_inline)) {
+        ra[set][i] = __builtin_amdgcn_raw_buffer_load_b128(a_rs, va[i], 0, 0);
+        va[i] += da;
         if constexpr (MASK) {
-            const u32x2u1 c = *reinterpret_cast<const u32x2u1*>(g.mask + row * g.ld_mask + om);
+            typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
+            const u32x2v c = __builtin_amdgcn_raw_buffer_load_b64(m_rs, vm[i], 0, 0);
             rm[set][i] = make_uint2(c[0], c[1]);
+            vm[i] += dm;
         }
     };
-    auto load_b = [&](auto last_c, int set, int i, int stage) __attribute__((always_inline)) {
-        constexpr bool LAST = decltype(last_c)::value;
-        const int64_t row = k0 + (int64_t)stage * kBigBK + (LAST ? 0 : BROWS * i);
-        uint32_t ob = vb, os = vs;
-        if constexpr (LAST) {
-            const int left = rows - stage * kBigBK - 1, r = brow + BROWS * i < left ? brow + BROWS * i : left;
-            ob = (uint32_t)(r * ldc + nb);
-            os = (uint32_t)(r * lds + nb / equss::kCkptBlock);
-        }
-        rb[set][i] = *reinterpret_cast<const u32x4a*>(g.codes + row * g.ld_codes + ob);
-        rs[set][i] = (g.scales + row * g.ld_scales)[os];
+    auto load_b = [&](int set, int i) __attribute__((always_inline)) {
+        rb[set][i] = __builtin_amdgcn_raw_buffer_load_b128(b_rs, vb[i], 0, 0);
+        rs[set][i] = __builtin_amdgcn_raw_buffer_load_b8(s_rs, vs[i], 0, 0);
+        vb[i] += db;
+        vs[i] += ds;
     };
     float bsum[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) bsum[j] = 0.f;
-    // the bias: every tile of a row of tiles adds up its share of the stages, [bias0, bias1); even ones, as the loop goes by two
-    const int bias0 = g.bias ? (int)((int64_t)stages * tn / g.tiles_n) & ~1 : 0;
-    const int bias1 = !g.bias ? 0 : tn + 1 == g.tiles_n ? stages : (int)((int64_t)stages * (tn + 1) / g.tiles_n) & ~1;
-    auto store_a = [&](auto last_c, auto bias_c, int set, int i, int stage, char* sb) __attribute__((always_inline)) {
-        const int r = arow + AROWS * i;
+    char* const wa = smem + arow * RA + ((ach ^ (4 * (arow & 3))) * 16);                 // (AROWS and BROWS are multiples of 4)
+    char* const wb0 = smem + kBigBK * RA + brow * RB + (((2 * bch) ^ (4 * (brow & 3))) * 16);
+    char* const wb1 = smem + kBigBK * RA + brow * RB + (((2 * bch + 1) ^ (4 * (brow & 3))) * 16);
+    auto store_a = [&](auto bias_c, int set, int i, int slot) __attribute__((always_inline)) {
         u32x4a v = ra[set][i];
         if constexpr (MASK) {
 #pragma unroll
@@ -294,33 +303,23 @@ __global__ __launch_bounds__(256, 1) void gemm_tn_ckpt_big_kernel(const Args g) 
                 v[j] &= ((int8_t)w > 0 ? 0xffffu : 0u) | ((int8_t)(w >> 8) > 0 ? 0xffff0000u : 0u);
             }
         }
-        if constexpr (decltype(last_c)::value) {
-            if (stage * kBigBK + r >= rows) v = u32x4a{0, 0, 0, 0};
-        }
         if constexpr (decltype(bias_c)::value) {
-            const uint32_t mine = !decltype(last_c)::value || (stage >= bias0 && stage < bias1) ? 0xffffffffu : 0u;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                bsum[2 * j] += equss::bits_as<float>((v[j] & mine) << 16);
-                bsum[2 * j + 1] += equss::bits_as<float>(v[j] & mine & 0xffff0000u);
+                bsum[2 * j] += equss::bits_as<float>(v[j] << 16);
+                bsum[2 * j + 1] += equss::bits_as<float>(v[j] & 0xffff0000u);
             }
         }
-        *reinterpret_cast<u32x4a*>(sb + r * RA + ((ach ^ (4 * (r & 3))) * 16)) = v;
+        *reinterpret_cast<u32x4a*>(wa + slot * SLOT + i * AROWS * RA) = v;
     };
-    auto store_b = [&](auto last_c, int set, int i, int stage, char* sb) __attribute__((always_inline)) {
-        const int r = brow + BROWS * i;
-        uint32_t sc = rs[set][i];
-        u32x4a c = rb[set][i];
-        if constexpr (decltype(last_c)::value) {
-            if (stage * kBigBK + r >= rows) { sc = 0; c = u32x4a{0, 0, 0, 0}; }
-        }
-        const float s = equss::ckpt_scale(sc);
-        char* row = sb + kBigBK * RA + r * RB;
-        *reinterpret_cast<u32x4a*>(row + (((2 * bch) ^ (4 * (r & 3))) * 16)) = to_bf16x8<E4M3>(c[0], c[1], s);
-        *reinterpret_cast<u32x4a*>(row + (((2 * bch + 1) ^ (4 * (r & 3))) * 16)) = to_bf16x8<E4M3>(c[2], c[3], s);
+    auto store_b = [&](int set, int i, int slot) __attribute__((always_inline)) {
+        const u32x4a c = rb[set][i];
+        const float s = equss::ckpt_scale(rs[set][i]);
+        *reinterpret_cast<u32x4a*>(wb0 + slot * SLOT + i * BROWS * RB) = to_bf16x8<E4M3>(c[0], c[1], s);
+        *reinterpret_cast<u32x4a*>(wb1 + slot * SLOT + i * BROWS * RB) = to_bf16x8<E4M3>(c[2], c[3], s);
     };
 
-    const int wm = wave >> 1, wn = wave & 1;
+    const int wm = wave / WAVES_N, wn = wave % WAVES_N;
     const int q = (lane >> 2) & 3, pp = lane & 3, hg = (lane >> 4) & 1, kb = lane >> 5;
     auto frag_at = [&](int c0, int row_bytes) __attribute__((always_inline)) {
         const int chunk = c0 / 8 + 2 * hg + (pp >> 1);
@@ -332,64 +331,52 @@ __global__ __launch_bounds__(256, 1) void gemm_tn_ckpt_big_kernel(const Args g) 
         const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(at + 4 * row_bytes));
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     };
-    int a_at[WM], b_at[WN];
+    const char *a_at[WM], *b_at[WNW];
 #pragma unroll
-    for (int t = 0; t < WM; ++t) a_at[t] = frag_at((wm * WM + t) * 32, RA);
+    for (int t = 0; t < WM; ++t) a_at[t] = smem + frag_at((wm * WM + t) * 32, RA);
 #pragma unroll
-    for (int t = 0; t < WN; ++t) b_at[t] = kBigBK * RA + frag_at((wn * WN + t) * 32, RB);
-    bf16x8 af[2][WM], bf[2][WN];
-    auto read = [&](int set, const char* slot, int ks) __attribute__((always_inline)) {
+    for (int t = 0; t < WNW; ++t) b_at[t] = smem + kBigBK * RA + frag_at((wn * WNW + t) * 32, RB);
+    bf16x8 af[2][WM], bf[2][WNW];
+    auto read = [&](int set, int slot, int ks) __attribute__((always_inline)) {
 #pragma unroll
-        for (int t = 0; t < WM; ++t) af[set][t] = frag(slot + ks * 16 * RA + a_at[t], RA);
+        for (int t = 0; t < WNW; ++t) bf[set][t] = frag(b_at[t] + slot * SLOT + ks * 16 * RB, RB);
 #pragma unroll
-        for (int t = 0; t < WN; ++t) bf[set][t] = frag(slot + ks * 16 * RB + b_at[t], RB);
+        for (int t = 0; t < WM; ++t) af[set][t] = frag(a_at[t] + slot * SLOT + ks * 16 * RA, RA);
     };
-    f32x16 acc[WM][WN];
+    f32x16 acc[WM][WNW];
 #pragma unroll
     for (int i = 0; i < WM; ++i)
 #pragma unroll
-        for (int j = 0; j < WN; ++j)
+        for (int j = 0; j < WNW; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
     auto multiply = [&](int set) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < WM; ++i)
 #pragma unroll
-            for (int j = 0; j < WN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[set][i], bf[set][j], acc[i][j], 0, 0, 0);
+            for (int j = 0; j < WNW; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[set][i], bf[set][j], acc[i][j], 0, 0, 0);
     };
     using No = std::false_type;
     using Yes = std::true_type;
-    auto fetch = [&](int set, int stage) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < AP; ++i) load_a(Yes(), set, i, stage);
-#pragma unroll
-        for (int i = 0; i < BP; ++i) load_b(Yes(), set, i, stage);
-    };
-    auto put = [&](int set, int stage, char* slot) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < AP; ++i) store_a(Yes(), Yes(), set, i, stage, slot);
-#pragma unroll
-        for (int i = 0; i < BP; ++i) store_b(Yes(), set, i, stage, slot);
-    };
-    // one stage: multiply `stage`, read ahead, store stage + 2 and request stage + 4 (which are there and whole)
-    auto step = [&](auto bias_c, int set, int stage, const char* s0, const char* s1, char* s2) __attribute__((always_inline)) {
-        const No last_c;
+    // one stage: multiply slot S, read ahead, store the stage after the next (register set S & 1) and request the one two behind it
+    auto step = [&](auto bias_c, auto slot_c) __attribute__((always_inline)) {
+        constexpr int S = decltype(slot_c)::value, SET = S & 1, S1 = (S + 1) & 3, S2 = (S + 2) & 3;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-            if (ks == 0) read(1, s0, 1);
-            else read(0, s1, 0);
+            if (ks == 0) read(1, S, 1);
+            else read(0, S1, 0);
 #pragma unroll
-            for (int i = ks * AP / 2; i < (ks + 1) * AP / 2; ++i) { store_a(last_c, bias_c, set, i, stage + 2, s2); load_a(last_c, set, i, stage + 4); }
+            for (int i = ks * AP / 2; i < (ks + 1) * AP / 2; ++i) { store_a(bias_c, SET, i, S2); load_a(SET, i); }
 #pragma unroll
-            for (int i = ks * BP / 2; i < (ks + 1) * BP / 2; ++i) { store_b(last_c, set, i, stage + 2, s2); load_b(last_c, set, i, stage + 4); }
+            for (int i = ks == 0 ? 0 : BP; i < BP; ++i) { store_b(SET, i, S2); load_b(SET, i); }
             multiply(ks);
-            // the order wanted: behind every MFMA two fragment reads (first half) or a store and its next request, and conversions
+            // the order wanted: behind every MFMA two fragment reads, conversions, and further on the stores and requests
 #pragma unroll
-            for (int i = 0; i < WM * WN; ++i) {
+            for (int i = 0; i < WM * WNW; ++i) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);            // MFMA
-                if (i < WM + WN) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);   // LDS reads
-                __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);            // VALU
-                if (i >= WM * WN / 2) {
+                if (i < WM + WNW) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);   // LDS reads
+                __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);            // VALU
+                if (i >= WM * WNW / 2) {
                     __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);        // LDS write
                     __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);        // global load
                 }
@@ -398,49 +385,72 @@ __global__ __launch_bounds__(256, 1) void gemm_tn_ckpt_big_kernel(const Args g) 
         }
         __syncthreads();
     };
-
-    if (stages > 0) {
-        fetch(0, 0);
-        if (stages > 1) fetch(1, 1);
-        put(0, 0, smem);
-        if (stages > 2) fetch(0, 2);
-        if (stages > 1) put(1, 1, smem + SLOT);
-        if (stages > 3) fetch(1, 3);
+    // the bias: each of the first `bias_tiles` tiles of a row of tiles adds up its share of the stages, [bias0, bias1); whole
+    // rounds of four
+    const int rounds = (stages + 3) / 4;
+    const bool adds = g.bias && tn < g.bias_tiles;
+    const int bias0 = adds ? (int)((int64_t)rounds * tn / g.bias_tiles) : 0;
+    const int bias1 = adds ? (int)((int64_t)rounds * (tn + 1) / g.bias_tiles) : 0;
+    {
+        // stages 0 and 1 into their slots, 2 and 3 requested
+        auto first = [&](auto bias_c) __attribute__((always_inline)) {
+#pragma unroll
+            for (int set = 0; set < 2; ++set) {
+#pragma unroll
+                for (int i = 0; i < AP; ++i) store_a(bias_c, set, i, set);
+#pragma unroll
+                for (int i = 0; i < BP; ++i) store_b(set, i, set);
+            }
+        };
+#pragma unroll
+        for (int set = 0; set < 2; ++set) {
+#pragma unroll
+            for (int i = 0; i < AP; ++i) load_a(set, i);
+#pragma unroll
+            for (int i = 0; i < BP; ++i) load_b(set, i);
+        }
+        if (bias0 == 0 && bias1 > 0) first(Yes());
+        else first(No());
+#pragma unroll
+        for (int set = 0; set < 2; ++set) {
+#pragma unroll
+            for (int i = 0; i < AP; ++i) load_a(set, i);
+#pragma unroll
+            for (int i = 0; i < BP; ++i) load_b(set, i);
+        }
     }
     __syncthreads();
-    if (stages > 0) read(0, smem, 0);
-    int stage = 0, slot = 0;
-    auto at = [&](int k) __attribute__((always_inline)) { return smem + (slot + k >= kSlots ? slot + k - kSlots : slot + k) * SLOT; };
-    auto next = [&]() __attribute__((always_inline)) {
-        ++stage;
-        slot = slot + 1 == kSlots ? 0 : slot + 1;
-    };
-    const int end = whole - 4;
-    auto run = [&](auto bias_c, int to) __attribute__((always_inline)) {
-        while (stage + 1 < to) {
-            step(bias_c, 0, stage, at(0), at(1), at(2));
-            next();
-            step(bias_c, 1, stage, at(0), at(1), at(2));
-            next();
+    read(0, 0, 0);
+    // A round stores stages 2 .. 5 of its own count, so the stores of [4 bias0, 4 bias1) are: the second half of round bias0 - 1
+    // (the start above for 0), the rounds from bias0 on, and the first half of round bias1 - 1.
+    using S0 = std::integral_constant<int, 0>;
+    using S1c = std::integral_constant<int, 1>;
+    using S2c = std::integral_constant<int, 2>;
+    using S3c = std::integral_constant<int, 3>;
+    int round = 0;
+    auto run = [&](auto first_half, auto second_half, int to) __attribute__((always_inline)) {
+        for (; round < to; ++round) {
+            step(first_half, S0());
+            step(first_half, S1c());
+            step(second_half, S2c());
+            step(second_half, S3c());
         }
     };
-    run(No(), end < bias0 - 2 ? end : bias0 - 2);
-    run(Yes(), end < bias1 - 2 ? end : bias1 - 2);
-    run(No(), end);
-    auto last = [&](int set) __attribute__((always_inline)) {                              // the last few, one thing after the other
-        if (stage + 2 < stages) put(set, stage + 2, at(2));
-        if (stage + 4 < stages) fetch(set, stage + 4);
-        read(1, at(0), 1);
-        multiply(0);
-        if (stage + 1 < stages) read(0, at(1), 0);
-        multiply(1);
-        __syncthreads();
-        next();
-    };
-    while (stage < stages) {
-        last(0);
-        if (stage < stages) last(1);
+    if (stages <= 2) {                                      // both are in LDS and counted: half a round
+        for (; round < rounds; ++round) {
+            step(No(), S0());
+            step(No(), S1c());
+        }
     }
+    if (adds) {
+        run(No(), No(), bias0 - 1);
+        if (bias1 > bias0) {
+            run(No(), Yes(), bias0);
+            run(Yes(), Yes(), bias1 - 1);
+            run(Yes(), No(), bias1);
+        }
+    }
+    run(No(), No(), rounds);
 
     float* c = g.c + split * g.split_c;
 #pragma unroll
@@ -451,14 +461,15 @@ __global__ __launch_bounds__(256, 1) void gemm_tn_ckpt_big_kernel(const Args g) 
             if (chunk < g.M) {
                 const int m = (chunk + 8 <= g.M ? chunk : g.M - 8) + 4 * kb + (r & 3);
 #pragma unroll
-                for (int j = 0; j < WN; ++j) {
-                    const int n = n0 + (wn * WN + j) * 32 + (lane & 31);
+                for (int j = 0; j < WNW; ++j) {
+                    const int n = n0 + (wn * WNW + j) * 32 + (lane & 31);
                     if (n < g.N) c[m * g.ldc + n] = acc[i][j][r];
                 }
             }
         }
-    if (g.bias) {
+    if (adds) {
         float* part = reinterpret_cast<float*>(smem);      // (every reader of the tiles is behind the loop's last barrier)
+        __syncthreads();
 #pragma unroll
         for (int j = 0; j < 8; ++j) part[arow * (8 * ACH) + 8 * ach + j] = bsum[j];
         __syncthreads();
@@ -466,7 +477,7 @@ __global__ __launch_bounds__(256, 1) void gemm_tn_ckpt_big_kernel(const Args g) 
         if (tid < TMB && chunk < g.M) {
             float s = 0.f;
             for (int r = 0; r < AROWS; ++r) s += part[r * (8 * ACH) + tid];
-            g.bias[(split * g.tiles_n + tn) * g.split_bias + (chunk + 8 <= g.M ? chunk : g.M - 8) + tid % 8] = s;
+            g.bias[(split * g.bias_tiles + tn) * g.split_bias + (chunk + 8 <= g.M ? chunk : g.M - 8) + tid % 8] = s;
         }
     }
 }
@@ -474,9 +485,9 @@ __global__ __launch_bounds__(256, 1) void gemm_tn_ckpt_big_kernel(const Args g) 
 // C = sum of the partial products, in the order of the splits; then the bias
 __global__ __launch_bounds__(256) void gemm_tn_join_kernel(const float* __restrict__ part, int64_t split_c, float* __restrict__ c,
                                                           int64_t ldc, const float* __restrict__ bpart, int64_t split_bias,
-                                                          float* __restrict__ bias, int splits, int bias_splits, int M, int N, int bias_len) {
+                                                          float* __restrict__ bias, int splits, int bias_splits, int M, int N) {
     const int64_t cells = (int64_t)M * N;
-    const int64_t total = cells + (bias ? bias_len : 0);
+    const int64_t total = cells + (bias ? M : 0);
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         const bool main = i < cells;
         const float* p = main ? part + i : bpart + (i - cells);
@@ -497,38 +508,54 @@ __global__ __launch_bounds__(256) void gemm_tn_join_kernel(const float* __restri
     }
 }
 
-struct Plan { bool big; int tiles_m, tiles_n, splits, bias_splits; int64_t rows_split; };
+struct Plan { int tile, tiles_m, tiles_n, splits, bias_splits; int64_t rows_split; };
 
-Plan plan(int64_t rows, int M, int N) {
+// 32-bit byte offsets within a workgroup's rows (and the eight stages that the loop may ask for behind them)
+bool offsets_fit(const Plan& p, int64_t ld_bytes) { return (p.rows_split + 8 * kBigBK) * ld_bytes < ((int64_t)1 << 31); }
+
+// tile 0: the narrow kernel (tiles of TM x TN)
+Plan plan(int64_t rows, int M, int N, int tile) {
     Plan p;
-    p.big = M > 128 && N > 128;
-    const int tm = p.big ? 256 : TM, tn = p.big ? 256 : TN, bk = p.big ? kBigBK : BK;
-    p.tiles_m = (M + tm - 1) / tm;
-    p.tiles_n = (N + tn - 1) / tn;
+    p.tile = tile;
+    const int t = tile ? tile : TM, bk = BK;
+    p.tiles_m = (M + t - 1) / t;
+    p.tiles_n = (N + t - 1) / t;
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-    int64_t splits = p.big ? 256 / tiles : (512 + tiles - 1) / tiles;
-    const int64_t most = (rows + 4 * bk - 1) / (4 * bk);          // at least four steps a workgroup
-    if (splits > most) splits = most;
+    // Row ranges: one more shortens everybody's loop (0.4 us for 32 rows) and adds a partial product to write and read back
+    // (8 M N bytes at 5 TB/s); the sum is least near splits^2 = 7800 rows / (M N).  At most one round of workgroups.
+    int64_t splits = 1;
+    const int64_t most = (tile == 256 ? 256 : 512) / tiles, steps = (rows + 4 * bk - 1) / (4 * bk);   // at least four steps a workgroup
+    while (splits < most && splits < steps && (splits + 1) * (splits + 1) * (double)M * N <= 7800.0 * (double)rows) ++splits;
     if (splits < 1) splits = 1;
     p.rows_split = ((rows + splits - 1) / splits + bk - 1) / bk * bk;
     if (p.rows_split < bk) p.rows_split = bk;
     p.splits = (int)((rows + p.rows_split - 1) / p.rows_split);
     if (p.splits < 1) p.splits = 1;
-    p.bias_splits = p.big ? p.splits * p.tiles_n : p.splits;
+    // (one row range: the first tile of a row of tiles adds all of the bias, and there is nothing to join)
+    p.bias_splits = tile && p.splits > 1 ? p.splits * p.tiles_n : p.splits;
     return p;
 }
 
-// partial products and, behind them, partial bias sums; nothing where one row range and one tile across write the results
+int tile_of(int64_t rows, int M, int N) {
+    if (M < 8) return 0;
+    // Measured (us, int8; 128 against 256): 25088 x 1024 x 768 64.9 / 62.7, 12544 x 1024 x 768 42.1 / 43.6, 102400 x 384 x 384
+    // 57.4 / 67.7, 102400 x 1024 x 768 217 / 164, 1024 x 1024 x 768 18.3 / 24.8: the large tile, which reads half as much LDS
+    // for a product, pays where every CU has a long way to go.
+    return (double)rows * M * N >= 2e10 && M > 128 && N > 128 ? 256 : 128;
+}
+
+// partial products and, behind them, partial bias sums; nothing where one row range writes the results
 size_t workspace(const Plan& p, int M, int N) {
-    const size_t c = p.splits == 1 ? 0 : (size_t)p.splits * M * N, b = p.bias_splits == 1 ? 0 : (size_t)p.bias_splits * M;
-    return (c + b) * sizeof(float);
+    return p.splits == 1 ? 0 : ((size_t)p.splits * M * N + (size_t)p.bias_splits * M) * sizeof(float);
 }
 
 }  // namespace
 
 extern "C" size_t equss_gemm_tn_ckpt_workspace_bytes(int64_t rows, int M, int N) {
     if (rows < 0 || M <= 0 || N <= 0) return 0;
-    return workspace(plan(rows, M, N), M, N);
+    // (the narrow kernel stands in where leading dimensions are too long for the others)
+    const size_t a = workspace(plan(rows, M, N, tile_of(rows, M, N)), M, N), b = workspace(plan(rows, M, N, 0), M, N);
+    return a > b ? a : b;
 }
 
 extern "C" int equss_gemm_tn_ckpt(const void* a, int64_t lda, const void* codes, int64_t ld_codes, const void* scales, int64_t ld_scales,
@@ -547,40 +574,43 @@ extern "C" int equss_gemm_tn_ckpt(const void* a, int64_t lda, const void* codes,
     if (rows > 0 && relu_codes && (ld_relu < g.mpad || (ld_relu % equss::kCkptBlock) != 0 || ((uintptr_t)relu_codes % 16) != 0))
         return equss::fail(EQUSS_E_ALIGN, "equss_gemm_tn_ckpt: mask codes 16-byte aligned with a leading dimension that is a multiple of 32 "
                            "and holds %d", g.mpad);
-    const Plan p = plan(rows, M, N);
-    const size_t need = workspace(p, M, N);
+    const size_t need = equss_gemm_tn_ckpt_workspace_bytes(rows, M, N);
+    Plan p = plan(rows, M, N, tile_of(rows, M, N));
+    if (p.tile && !(offsets_fit(p, lda * 2) && offsets_fit(p, ld_codes) && offsets_fit(p, ld_scales) && offsets_fit(p, relu_codes ? ld_relu : 0)))
+        p = plan(rows, M, N, 0);
     if (need > 0 && (!workspace_ptr || workspace_bytes < need || ((uintptr_t)workspace_ptr % 16) != 0))
         return equss::fail(EQUSS_E_WORKSPACE, "equss_gemm_tn_ckpt: workspace of %zu bytes, 16-byte aligned, needed", need);
     const int64_t blocks = (int64_t)p.tiles_m * p.tiles_n * p.splits;
     if (blocks > 0x7fffffff || (p.rows_split + BK - 1) / BK > 0x7fffffff)
         return equss::fail(EQUSS_E_UNSUPPORTED, "equss_gemm_tn_ckpt: %lld rows, M=%d N=%d", (long long)rows, M, N);
-    // (offsets within a stage of 64 rows are 32 bits)
-    if (rows > 0 && (lda > (1 << 23) || ld_codes > (1 << 23) || ld_relu > (1 << 23)))
-        return equss::fail(EQUSS_E_UNSUPPORTED, "equss_gemm_tn_ckpt: a leading dimension exceeds %d", 1 << 23);
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     g.a = reinterpret_cast<const u16*>(a); g.lda = lda;
     g.codes = reinterpret_cast<const uint8_t*>(codes); g.ld_codes = ld_codes;
     g.scales = reinterpret_cast<const uint8_t*>(scales); g.ld_scales = ld_scales;
     g.mask = reinterpret_cast<const uint8_t*>(relu_codes); g.ld_mask = ld_relu;
-    g.rows = rows; g.rows_split = p.rows_split; g.M = M; g.N = N; g.tiles_m = p.tiles_m; g.tiles_n = p.tiles_n; g.splits = p.splits;
+    g.rows = rows; g.rows_split = p.rows_split; g.M = M; g.N = N; g.tiles_m = p.tiles_m; g.tiles_n = p.tiles_n; g.splits = p.splits; g.bias_tiles = p.bias_splits / p.splits;
     float* part = reinterpret_cast<float*>(workspace_ptr);
-    float* bpart = part + (p.splits == 1 ? 0 : (size_t)p.splits * M * N);
-    const bool direct = p.splits == 1, bias_direct = p.bias_splits == 1;
+    float* bpart = part + (size_t)p.splits * M * N;
+    const bool direct = p.splits == 1;
     g.c = direct ? C : part; g.ldc = direct ? ldc : N; g.split_c = direct ? 0 : (int64_t)M * N;
-    g.bias = bias ? (bias_direct ? bias : bpart) : nullptr; g.split_bias = M;
+    g.bias = bias ? (direct ? bias : bpart) : nullptr; g.split_bias = M;
     const bool e = fmt == EQUSS_CKPT_E4M3;
-    if (p.big) {
-        const int lds = kSlots * kBigBK * 1024;
+    if (p.tile) {
         const dim3 grid((unsigned)((blocks + 7) / 8 * 8));
-#define EQUSS_TN_BIG(E, K)                                                                                                     \
+        const int lds = kSlots * kBigBK * 4 * p.tile;
+#define EQUSS_TN_TILE(E, K, T)                                                                                                 \
     do {                                                                                                                       \
-        if (!equss::lds_opt_in(reinterpret_cast<const void*>(&gemm_tn_ckpt_big_kernel<E, K, 4, 4>), lds))                      \
+        if (!equss::lds_opt_in(reinterpret_cast<const void*>(&gemm_tn_ckpt_tile_kernel<E, K, T>), lds))                        \
             return equss::fail(EQUSS_E_UNSUPPORTED, "equss_gemm_tn_ckpt: %d bytes of LDS", lds);                               \
-        hipLaunchKernelGGL((gemm_tn_ckpt_big_kernel<E, K, 4, 4>), grid, dim3(256), lds, s, g);                                 \
+        hipLaunchKernelGGL((gemm_tn_ckpt_tile_kernel<E, K, T>), grid, dim3(2 * T), lds, s, g);                                 \
     } while (0)
-        if (e) { if (relu_codes) EQUSS_TN_BIG(true, true); else EQUSS_TN_BIG(true, false); }
-        else { if (relu_codes) EQUSS_TN_BIG(false, true); else EQUSS_TN_BIG(false, false); }
-#undef EQUSS_TN_BIG
+#define EQUSS_TN_FORM(T)                                                                                                       \
+    if (e) { if (relu_codes) EQUSS_TN_TILE(true, true, T); else EQUSS_TN_TILE(true, false, T); }                               \
+    else { if (relu_codes) EQUSS_TN_TILE(false, true, T); else EQUSS_TN_TILE(false, false, T); }
+        if (p.tile == 256) { EQUSS_TN_FORM(256) }
+        else { EQUSS_TN_FORM(128) }
+#undef EQUSS_TN_FORM
+#undef EQUSS_TN_TILE
     } else {
         const dim3 grid((unsigned)blocks), block(kTnThreads);
         if (e) {
@@ -592,13 +622,11 @@ extern "C" int equss_gemm_tn_ckpt(const void* a, int64_t lda, const void* codes,
         }
     }
     const int rc = equss::check_launch("gemm_tn_ckpt_kernel");
-    const bool join_bias = bias && !bias_direct;
-    if (rc != EQUSS_OK || (direct && !join_bias)) return rc;
-    // (with one row range the products are in place and only the bias is left)
-    const int64_t total = (direct ? 0 : (int64_t)M * N) + (join_bias ? M : 0);
-    int64_t gx = (total + 255) / 256;
+    if (rc != EQUSS_OK || direct) return rc;
+    const int64_t join = (int64_t)M * N + (bias ? M : 0);
+    int64_t gx = (join + 255) / 256;
     if (gx > 4096) gx = 4096;
-    hipLaunchKernelGGL(gemm_tn_join_kernel, dim3((unsigned)gx), dim3(256), 0, s, part, (int64_t)M * N, C, ldc, bpart, (int64_t)M,
-                       join_bias ? bias : nullptr, p.splits, p.bias_splits, direct ? 0 : M, direct ? 1 : N, M);
+    hipLaunchKernelGGL(gemm_tn_join_kernel, dim3((unsigned)gx), dim3(256), 0, s, part, (int64_t)M * N, C, ldc, bpart, (int64_t)M, bias, p.splits,
+                       p.bias_splits, M, N);
     return equss::check_launch("gemm_tn_join_kernel");
 }

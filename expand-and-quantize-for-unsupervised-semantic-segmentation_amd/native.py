@@ -205,10 +205,17 @@ def _stream(t):
     """The current HIP stream of ``t``'s device.  Kernels launch on the CURRENT device, so that device
     must be the tensor's: a launch with a foreign device's pointers and stream handle would corrupt
     memory silently, hence the loud failure (one process per GPU, as torchrun sets it up, never trips it)."""
-    if t.device.index is not None and t.device.index != torch.cuda.current_device():
+    index = t.device.index
+    if index is not None and index != torch.cuda.current_device():
         raise EqussError(f"tensor lives on {t.device} but the current device is cuda:{torch.cuda.current_device()}; "
                          f"wrap the call in `with torch.cuda.device({t.device.index}):`")
+    if _raw_stream is not None and index is not None:
+        return ctypes.c_void_p(_raw_stream(index))
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+# the current stream's handle without the Stream object around it (0.2 us instead of 2 us a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _ptr(t):

@@ -127,7 +127,8 @@ def whole_numbers(rows, width, fmt, seed, dev, native):
 
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 @pytest.mark.parametrize("rows,m,n", [(1, 1, 1), (1, 384, 384), (31, 8, 40), (33, 128, 128), (64, 130, 257), (129, 384, 96), (300, 1, 500),
-                                      (257, 500, 1), (1000, 200, 333), (4099, 129, 31), (2500, 1024, 768)])
+                                      (257, 500, 1), (1000, 200, 333), (4099, 129, 31), (2500, 1024, 768),
+                                      (300, 7, 200), (300, 8, 200), (900, 257, 130), (40, 131, 1000), (8000, 9, 20), (30000, 259, 301)])
 def test_weight_gradient_is_exact_on_whole_numbers(rows, m, n, fmt, native, dev):
     """Products and sums of whole numbers below 2^24 are exact in fp32 whatever their order: any difference is an element in the
     wrong place.  With and without the ReLU mask, with and without the bias."""
@@ -174,7 +175,9 @@ def test_weight_gradient_takes_views_and_no_rows(native, dev):
     g = torch.Generator().manual_seed(4)
     big = torch.randint(-2, 3, (500, 300), generator=g).to(torch.bfloat16).to(dev)
     v, kept = whole_numbers(500, 256, "int8", 6, dev, native)
-    for a in (big[:, 7:135], big[:, 3:10], big.t().contiguous().t()[:, :64]):
+    odd = torch.empty(500, 301, dtype=torch.bfloat16, device=dev)
+    odd[:, 1:] = big
+    for a in (big[:, 7:135], big[:, 3:10], big.t().contiguous().t()[:, :64], odd[:, 1:], odd[:, 2:160], odd[:, 5:12]):
         for lo, hi in ((0, 256), (64, 128), (224, 256)):
             got = native.gemm_tn_ckpt(a, kept.columns(lo, hi))
             assert torch.equal(got.cpu(), (a.cpu().to(F64).t() @ v[:, lo:hi].to(F64)).to(F32))
