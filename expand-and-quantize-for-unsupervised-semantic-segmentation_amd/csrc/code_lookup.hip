@@ -121,9 +121,9 @@ struct GradOp {
     float scale;
     int d;
     typedef f32x4 Row;
-    struct Code {};
-    __device__ __forceinline__ Row load(uint32_t row, int p, int col) const {
-        const typename Elem<T>::type* s = g + (int64_t)row * ld + (int64_t)p * d + col;
+    static constexpr bool kOwn = false;
+    __device__ __forceinline__ Row load(const equss::CodePair& at, int p, int col) const {
+        const typename Elem<T>::type* s = g + (int64_t)at.row * ld + (int64_t)p * d + col;
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
         if (col + 4 <= d) {
             if constexpr (T == 0) {
@@ -146,8 +146,8 @@ struct GradOp {
         }
         return v;
     }
-    __device__ __forceinline__ Code code(int, uint32_t, int) const { return Code{}; }
-    __device__ __forceinline__ f32x4 value(const Row& r, const Code&, uint32_t, int, int, bool) const { return r * scale; }
+    __device__ __forceinline__ f32x4 value(Row& r) const { return r * scale; }
+    __device__ __forceinline__ void own(const Row&, uint32_t, int, int) const {}
 };
 
 int index_checks(const char* what, const void* idx, int index_type, int64_t rows, int num_pq, int64_t K, int d, int type) {
@@ -164,13 +164,13 @@ int index_checks(const char* what, const void* idx, int index_type, int64_t rows
 template <int T>
 int grad(const void* g, int64_t ld, float scale, const equss::SortPlan& s, const equss::IndexView& index, char* ws, float* out, int d, hipStream_t stream) {
     const GradOp<T> op = {reinterpret_cast<const typename Elem<T>::type*>(g), ld, scale, d};
-    if (d <= 4) return equss::walk_launch_lpr<GradOp<T>, 1>(op, s, index, ws, out, d, false, stream);
-    if (d <= 8) return equss::walk_launch_lpr<GradOp<T>, 2>(op, s, index, ws, out, d, false, stream);
-    if (d <= 16) return equss::walk_launch_lpr<GradOp<T>, 4>(op, s, index, ws, out, d, false, stream);
-    if (d <= 32) return equss::walk_launch_lpr<GradOp<T>, 8>(op, s, index, ws, out, d, false, stream);
-    if (d <= 64) return equss::walk_launch_lpr<GradOp<T>, 16>(op, s, index, ws, out, d, false, stream);
-    if (d <= 128) return equss::walk_launch_lpr<GradOp<T>, 32>(op, s, index, ws, out, d, false, stream);
-    return equss::walk_launch_lpr<GradOp<T>, 64>(op, s, index, ws, out, d, false, stream);
+    if (d <= 4) return equss::walk_launch_lpr<GradOp<T>, 1>(op, s, index, ws, out, d, stream);
+    if (d <= 8) return equss::walk_launch_lpr<GradOp<T>, 2>(op, s, index, ws, out, d, stream);
+    if (d <= 16) return equss::walk_launch_lpr<GradOp<T>, 4>(op, s, index, ws, out, d, stream);
+    if (d <= 32) return equss::walk_launch_lpr<GradOp<T>, 8>(op, s, index, ws, out, d, stream);
+    if (d <= 64) return equss::walk_launch_lpr<GradOp<T>, 16>(op, s, index, ws, out, d, stream);
+    if (d <= 128) return equss::walk_launch_lpr<GradOp<T>, 32>(op, s, index, ws, out, d, stream);
+    return equss::walk_launch_lpr<GradOp<T>, 64>(op, s, index, ws, out, d, stream);
 }
 
 }  // namespace

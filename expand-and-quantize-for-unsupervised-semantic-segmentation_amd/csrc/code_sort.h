@@ -11,8 +11,10 @@
 //              tile borders leaves a partial sum on each
 //   join       the partial sums of a run in the order of the tiles, and zeros for codes without rows
 //
-// Up to kSmallRows rows all of it is one kernel (small): a workgroup owns a few codes, picks their rows out of all indices by
-// itself, in order, and sums them.
+// For few rows all of it is one kernel (small): a workgroup owns a few codes, picks their rows out of all indices by itself, in
+// order, and sums them.  Measured (us, gradient of a lookup, small against sorted): 1000 rows, 8 x 256 x 128: 12 / 23; 2048 rows:
+// 16 / 25, and 40 / 26 where every row has the same code; 4096 rows: 22 / 22 (92 / 29 with one code); 4096 rows, 16384 x 16,
+// whose sort takes two passes: 12 / 38.  Hence up to 2048 rows, and up to 4096 where the sort would take more than one pass.
 //
 // An index outside [0, K) counts as the code K, which sorts last and has no sum.
 #pragma once
@@ -35,10 +37,31 @@ __device__ __forceinline__ uint32_t code_at(const IndexView& v, int p, int64_t r
     return k >= 0 && k < (int64_t)K ? (uint32_t)k : K;
 }
 
+// The codes of rows r, r + step, ... (N of them; those past `end` give the last row's): the loads of one type side by side, so
+// that they wait once, not N times.
+template <int N>
+__device__ __forceinline__ void codes_at(const IndexView& v, int p, int64_t r, int step, int64_t end, uint32_t K, uint32_t (&code)[N]) {
+    int64_t k[N];
+    auto load = [&](auto* base) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int64_t at = r + (int64_t)j * step < end ? r + (int64_t)j * step : end - 1;
+            k[j] = base[at * v.stride_r];
+        }
+    };
+    const int64_t first = (int64_t)p * v.stride_p;
+    if (v.type == EQUSS_I64) load(reinterpret_cast<const int64_t*>(v.p) + first);
+    else if (v.type == EQUSS_I32) load(reinterpret_cast<const int32_t*>(v.p) + first);
+    else load(reinterpret_cast<const int16_t*>(v.p) + first);
+#pragma unroll
+    for (int j = 0; j < N; ++j) code[j] = k[j] >= 0 && k[j] < (int64_t)K ? (uint32_t)k[j] : K;
+}
+
 struct CodePair { uint32_t code, row; };
 
-constexpr int kSmallRows = 2048;
+constexpr int kSmallRows = 4096;        // most rows of the one-kernel form
 constexpr int kMaxBins = 2048;          // bins of a pass: 11 bits
+constexpr int kTile = 64;               // pairs of a tile, where there are enough of them
 
 // What a call sorts with; everything but `index` lies in the caller's workspace.
 struct SortPlan {
@@ -59,10 +82,10 @@ int sort_launch(const SortPlan& s, const IndexView& index, char* ws, size_t* pai
 
 // --------------------------------------------------------------------------------------------------------------------------
 // The walk.  Op gives the kernels their rows:
-//   struct Row;                                    what is loaded of one (row, p, lane)
-//   Row  load(row, p, col) const                   its loads
-//   struct Code; Code code(p, k, col) const        what it needs of the codeword (k == K: none)
-//   f32x4 value(const Row&, const Code&, row, p, col) const     the lane's four terms of the sum; may write the row's own output
+//   struct Row;                             what is loaded of one (code, row) pair and lane
+//   Row  load(pair, p, col) const           its loads
+//   f32x4 value(const Row&) const           the lane's four terms of the sum
+//   kOwn; void own(const Row&, row, p, col) whether there is one, and the row's own output, if it has one; after value(), which may keep what it needs in Row
 // A row's part of d elements is walked by LPR lanes with four elements each (d <= 4 LPR; beyond 256 in chunks of 256 columns).
 
 struct WalkArgs {
@@ -84,9 +107,11 @@ __device__ __forceinline__ void store_cols(float* p, f32x4 v, int col, int d, bo
     }
 }
 
-template <class Op, int LPR>
+// U: pairs in flight a group.  One where the chip is full of groups (102400 rows, 8 x 256 x 128, the quantiser's backward: 223 us
+// with 1, 251 with 2, 267 with 4), two where it is not (4096 rows: 33 / 30 / 31 us).
+template <class Op, int LPR, int U>
 __global__ __launch_bounds__(256) void code_accumulate_kernel(const Op op, const WalkArgs w) {
-    constexpr int SLOTS = 64 / LPR, U = 4;
+    constexpr int SLOTS = 64 / LPR;
     const int lane = threadIdx.x & 63;
     const int64_t tile = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * SLOTS + lane / LPR;
     if (tile >= w.tiles) return;                          // (whole groups of LPR lanes leave together)
@@ -99,15 +124,26 @@ __global__ __launch_bounds__(256) void code_accumulate_kernel(const Op op, const
     float* part = w.partial + (((int64_t)p * w.tiles + tile) * 2) * w.dpad + col;
     float* out = w.out + ((int64_t)p * w.K) * w.d + col;
     const bool sums = w.out != nullptr;
-    typename Op::Code code = op.code(p, cur, live ? col : 0);
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    CodePair next[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) next[j] = pairs[t0 + j < t1 ? t0 + j : t1 - 1];
     for (int64_t i = t0; i < t1; i += U) {
         CodePair pr[U];
         typename Op::Row row[U];
+        f32x4 v[U];
 #pragma unroll
-        for (int j = 0; j < U; ++j) pr[j] = pairs[i + j < t1 ? i + j : t1 - 1];
+        for (int j = 0; j < U; ++j) {
+            pr[j] = next[j];
+            row[j] = op.load(pr[j], p, live ? col : 0);
+        }
 #pragma unroll
-        for (int j = 0; j < U; ++j) row[j] = op.load(pr[j].row, p, live ? col : 0);
+        for (int j = 0; j < U; ++j) next[j] = pairs[i + U + j < t1 ? i + U + j : t1 - 1];
+        // (a pair past the tile's end is its last one again: its value is not used and its own output is the same once more)
+#pragma unroll
+        for (int j = 0; j < U; ++j) v[j] = op.value(row[j]);
+#pragma unroll
+        for (int j = 0; j < U; ++j) op.own(row[j], pr[j].row, p, col);
 #pragma unroll
         for (int j = 0; j < U; ++j) {
             if (i + j < t1) {
@@ -118,10 +154,9 @@ __global__ __launch_bounds__(256) void code_accumulate_kernel(const Op op, const
                     }
                     head = false;
                     cur = pr[j].code;
-                    code = op.code(p, cur, live ? col : 0);
                     acc = f32x4{0.f, 0.f, 0.f, 0.f};
                 }
-                acc += op.value(row[j], code, pr[j].row, p, col, live);
+                acc += v[j];
             }
         }
     }
@@ -147,15 +182,28 @@ __global__ __launch_bounds__(256) void code_join_kernel(const WalkArgs w) {
     // link 0 is the first tile's tail, the others the following tiles' heads; sums of links first, first + step, ...
     auto chain = [&](int64_t ts, int64_t links, int64_t first, int64_t step) {
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-        for (int64_t j = first; j < links; j += step)
-            acc += *reinterpret_cast<const f32x4*>(part + ((ts + j) * 2 + (j == 0 ? 1 : 0)) * w.dpad);
+        for (int64_t j = first; j < links; j += 4 * step) {
+            f32x4 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t l = j + i * step < links ? j + i * step : first;
+                v[i] = *reinterpret_cast<const f32x4*>(part + ((ts + l) * 2 + (l == 0 ? 1 : 0)) * w.dpad);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (j + i * step < links) acc += v[i];
+        }
         return acc;
     };
     const int64_t k0 = (int64_t)blockIdx.x * 4;
+    int64_t at[5];
+#pragma unroll
+    for (int c = 0; c < 5; ++c) at[c] = starts[k0 + c <= (int64_t)w.K ? k0 + c : (int64_t)w.K];
+#pragma unroll
     for (int c = 0; c < 4; ++c) {
         const int64_t k = k0 + c;
         if (k >= (int64_t)w.K) break;                      // (uniform over the workgroup)
-        const int64_t s = starts[k], e = starts[k + 1];
+        const int64_t s = at[c], e = at[c + 1];
         const int64_t ts = s / w.tile, links = e > s ? (e - 1) / w.tile - ts + 1 : 0;
         const bool far = links > kLong;
         if (!far) {
@@ -179,53 +227,144 @@ __global__ __launch_bounds__(256) void code_join_kernel(const WalkArgs w) {
     }
 }
 
-// All in one for few rows: the workgroup's codes are [k0, k0 + codes); `rest` tells the last workgroup to walk the rows
-// without a code too (for their own outputs).
-template <class Op, int LPR>
+// All in one for few rows: the workgroup's codes are [k0, k0 + codes).  Its rows come out of the indices in row order, eight
+// indices a thread at a time, and are put in the order of their codes by a bitonic sort of (code, row) where they are few
+// (256, a thread each); groups of lanes then walk the codes, several to a code where there are more groups than codes.  Where
+// one code has most of the rows, everybody walks the unsorted list once for each code.  The last workgroup has the rows without a
+// code too, for their own outputs.
+template <class Op, int LPR, int CAP>                     // CAP: most rows
 __global__ __launch_bounds__(256) void code_small_kernel(const Op op, const IndexView index, float* __restrict__ out_all, int rows,
-                                                        uint32_t K, int d, int codes, int rest) {
-    constexpr int SLOTS = 256 / LPR;
-    __shared__ CodePair list[kSmallRows];
+                                                        uint32_t K, int d, int codes) {
+    constexpr int SLOTS = 256 / LPR, PER = 8, FLIGHT = Op::kOwn ? 4 : 8;
+    __shared__ CodePair list[CAP];
     __shared__ f32x4 share[256];
-    __shared__ int wave_count[4];
+    __shared__ int wave_count[PER][4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, slot = tid / LPR;
     const int p = blockIdx.y, col = (int)blockIdx.z * 256 + (tid % LPR) * 4;
     const bool live = col < d, whole = (d & 3) == 0;
     const uint32_t k0 = blockIdx.x * (uint32_t)codes;
-    uint32_t k1 = k0 + codes < K ? k0 + codes : K;
-    const uint32_t kend = k1;
-    if (rest && blockIdx.x == gridDim.x - 1) k1 = K + 1;
+    const uint32_t kend = k0 + codes < K ? k0 + codes : K;
+    const uint32_t k1 = blockIdx.x == gridDim.x - 1 ? K + 1 : kend;
     int count = 0;
-    for (int r0 = 0; r0 < rows; r0 += 256) {
-        const int r = r0 + tid;
-        uint32_t k = 0;
-        bool mine = false;
-        if (r < rows) {
-            k = code_at(index, p, r, K);
-            mine = k >= k0 && k < k1;
+    for (int r0 = 0; r0 < rows; r0 += 256 * PER) {
+        uint32_t k[PER];
+        uint64_t m[PER];
+        codes_at<PER>(index, p, r0 + tid, 256, rows, K, k);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            if (r0 + j * 256 + tid >= rows) k[j] = k1;
+            m[j] = __ballot(k[j] >= k0 && k[j] < k1);
+            if (lane == 0) wave_count[j][wave] = __popcll(m[j]);
         }
-        const uint64_t m = __ballot(mine);
-        if (lane == 0) wave_count[wave] = __popcll(m);
         __syncthreads();
-        int at = count;
-        for (int i = 0; i < 4; ++i) {
-            if (i < wave) at += wave_count[i];
-            count += wave_count[i];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            int at = count;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (i < wave) at += wave_count[j][i];
+                count += wave_count[j][i];
+            }
+            if (k[j] >= k0 && k[j] < k1) list[at + __popcll(m[j] & ((1ull << lane) - 1))] = CodePair{k[j], (uint32_t)(r0 + j * 256 + tid)};
         }
-        if (mine) list[at + __popcll(m & ((1ull << lane) - 1))] = CodePair{k, (uint32_t)r};
         __syncthreads();
     }
     float* out = out_all + (int64_t)p * K * d + col;
     const bool sums = out_all != nullptr;
-    const int lo = (int)((int64_t)count * slot / SLOTS), hi = (int)((int64_t)count * (slot + 1) / SLOTS);
-    for (uint32_t k = k0; k < k1; ++k) {
-        const typename Op::Code code = op.code(p, k, live ? col : 0);
+    auto sum_range = [&](int lo, int hi) {
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-        for (int j = lo; j < hi; ++j)
-            if (list[j].code == k) {
-                const uint32_t r = list[j].row;
-                acc += op.value(op.load(r, p, live ? col : 0), code, r, p, col, live);
+        for (int j = lo; j < hi; j += 4) {
+            typename Op::Row row[4];
+            f32x4 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) row[i] = op.load(list[j + i < hi ? j + i : hi - 1], p, live ? col : 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = op.value(row[i]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (j + i < hi) {
+                    acc += v[i];
+                    op.own(row[i], list[j + i].row, p, col);
+                }
+        }
+        return acc;
+    };
+    if (count <= 256) {
+        // codes of this workgroup fit 16 bits beside the row's 11 only where they are few; 64-bit keys always do
+        uint64_t key = tid < count ? (uint64_t)list[tid].code << 32 | list[tid].row : ~0ull;
+        for (int width = 2; width <= 256; width *= 2) {
+            if (width / 2 >= count) break;                 // (uniform: everything behind `count` is the largest key already)
+            for (int step = width / 2; step > 0; step /= 2) {
+                uint64_t other;
+                if (step < 64) other = (uint64_t)__shfl_xor((long long)key, step, 64);
+                else {
+                    uint64_t* keys = reinterpret_cast<uint64_t*>(share);
+                    keys[tid] = key;
+                    __syncthreads();
+                    other = keys[tid ^ step];
+                    __syncthreads();
+                }
+                const bool up = (tid & width) == 0, low = (tid & step) == 0;
+                key = (up == low) == (key < other) ? key : other;
             }
+        }
+        if (tid < count) list[tid] = CodePair{(uint32_t)(key >> 32), (uint32_t)key};
+        __syncthreads();
+        auto first_of = [&](uint32_t k) {                  // the first entry whose code is not below k
+            int lo = 0, hi = count;
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (list[mid].code < k) lo = mid + 1;
+                else hi = mid;
+            }
+            return lo;
+        };
+        const int n = (int)(k1 - k0);
+        const int parts = n < SLOTS ? SLOTS / n : 1;       // groups that share a code
+        for (int c0 = 0; c0 < n; c0 += SLOTS / parts) {
+            const int c = c0 + slot / parts, part = slot % parts;
+            const bool mine = slot / parts < SLOTS / parts && c < n;
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+            if (mine) {
+                const int lo = first_of(k0 + c), hi = first_of(k0 + c + 1), len = hi - lo;
+                if (Op::kOwn || k0 + c < kend) acc = sum_range(lo + len * part / parts, lo + len * (part + 1) / parts);
+            }
+            if (!sums) continue;
+            if (parts > 1) {                               // (then there is one round)
+                share[tid] = acc;
+                __syncthreads();
+                if (mine && part == 0)
+                    for (int j = 1; j < parts; ++j) acc += share[tid + j * LPR];
+            }
+            if (mine && part == 0 && live && k0 + c < kend) store_cols(out + (int64_t)(k0 + c) * d, acc, col, d, whole);
+        }
+        return;
+    }
+    // (several rows in flight where any of their entries has the code: one codeword may own all the rows)
+    const int lo = (int)((int64_t)count * slot / SLOTS), hi = (int)((int64_t)count * (slot + 1) / SLOTS);
+    for (uint32_t k = k0; k < (Op::kOwn ? k1 : kend); ++k) {
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int j = lo; j < hi; j += FLIGHT) {
+            CodePair pr[FLIGHT];
+            bool any = false;
+#pragma unroll
+            for (int i = 0; i < FLIGHT; ++i) {
+                pr[i] = list[j + i < hi ? j + i : hi - 1];
+                any |= pr[i].code == k;
+            }
+            if (!any) continue;
+            typename Op::Row row[FLIGHT];
+#pragma unroll
+            for (int i = 0; i < FLIGHT; ++i) row[i] = op.load(pr[i], p, live ? col : 0);
+#pragma unroll
+            for (int i = 0; i < FLIGHT; ++i) {
+                const f32x4 v = op.value(row[i]);
+                if (j + i < hi && pr[i].code == k) {
+                    acc += v;
+                    op.own(row[i], pr[i].row, p, col);
+                }
+            }
+        }
         if (!sums || k >= kend) continue;                  // (uniform)
         share[tid] = acc;
         __syncthreads();
@@ -238,15 +377,18 @@ __global__ __launch_bounds__(256) void code_small_kernel(const Op op, const Inde
 }
 
 template <class Op, int LPR>
-int walk_launch_lpr(const Op& op, const SortPlan& s, const IndexView& index, char* ws, float* out, int d, bool rest, hipStream_t stream) {
+int walk_launch_lpr(const Op& op, const SortPlan& s, const IndexView& index, char* ws, float* out, int d, hipStream_t stream) {
     const unsigned cchunks = (unsigned)((d + 255) / 256);
     if (s.passes == 0) {
         // codes a workgroup: about a thousand workgroups
         int64_t codes = ((int64_t)s.K * s.num_pq + 1023) / 1024;
         if (codes < 1) codes = 1;
         const unsigned gx = (unsigned)(((int64_t)s.K + codes - 1) / codes);
-        hipLaunchKernelGGL((code_small_kernel<Op, LPR>), dim3(gx, s.num_pq, cchunks), dim3(256), 0, stream, op, index, out, (int)s.rows, s.K,
-                           d, (int)codes, rest ? 1 : 0);
+        const dim3 grid(gx, s.num_pq, cchunks);
+        if (s.rows <= kSmallRows / 2)
+            hipLaunchKernelGGL((code_small_kernel<Op, LPR, kSmallRows / 2>), grid, dim3(256), 0, stream, op, index, out, (int)s.rows, s.K, d, (int)codes);
+        else
+            hipLaunchKernelGGL((code_small_kernel<Op, LPR, kSmallRows>), grid, dim3(256), 0, stream, op, index, out, (int)s.rows, s.K, d, (int)codes);
         return check_launch("code_small_kernel");
     }
     size_t at = 0;
@@ -258,8 +400,9 @@ int walk_launch_lpr(const Op& op, const SortPlan& s, const IndexView& index, cha
     w.partial = reinterpret_cast<float*>(ws + s.partial);
     w.out = out; w.rows = s.rows; w.tiles = s.tiles; w.tile = s.tile; w.d = d; w.dpad = (d + 3) / 4 * 4; w.K = s.K;
     constexpr int TILES_WG = 4 * (64 / LPR);
-    hipLaunchKernelGGL((code_accumulate_kernel<Op, LPR>), dim3((unsigned)((s.tiles + TILES_WG - 1) / TILES_WG), s.num_pq, cchunks), dim3(256), 0,
-                       stream, op, w);
+    const dim3 grid((unsigned)((s.tiles + TILES_WG - 1) / TILES_WG), s.num_pq, cchunks);
+    if (s.tile == kTile) hipLaunchKernelGGL((code_accumulate_kernel<Op, LPR, 1>), grid, dim3(256), 0, stream, op, w);
+    else hipLaunchKernelGGL((code_accumulate_kernel<Op, LPR, 2>), grid, dim3(256), 0, stream, op, w);
     rc = check_launch("code_accumulate_kernel");
     if (rc != EQUSS_OK || !out) return rc;
     hipLaunchKernelGGL((code_join_kernel<LPR>), dim3((s.K + 3) / 4, s.num_pq, cchunks), dim3(256), 0, stream, w);

@@ -5,6 +5,7 @@
 #include <stdint.h>
 #include <stdio.h>
 #include <stdarg.h>
+#include <type_traits>
 #include "../../include/equss_hip.h"
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -186,6 +187,24 @@ template <int WIDTH>
 __device__ __forceinline__ float group_sum(float v) {  // sum over WIDTH consecutive lanes
 #pragma unroll
     for (int off = WIDTH / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+    return v;
+}
+// The same sum over 4, 8, 16 or 32 lanes without LDS: lane exchanges inside rows of 16 are operands of the addition (DPP), and
+// the two rows of 32 lanes exchange by v_permlane16_swap.
+template <int WIDTH>
+__device__ __forceinline__ float lanes_sum(float v) {
+    static_assert(WIDTH == 4 || WIDTH == 8 || WIDTH == 16 || WIDTH == 32, "");
+    auto dpp = [](float x, auto ctrl) {
+        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, 0xf, 0xf, true));
+    };
+    v += dpp(v, std::integral_constant<int, 0xb1>());                          // quad_perm 1 0 3 2
+    v += dpp(v, std::integral_constant<int, 0x4e>());                          // quad_perm 2 3 0 1
+    if constexpr (WIDTH >= 8) v += dpp(v, std::integral_constant<int, 0x141>());   // the other quad of eight lanes (mirrored)
+    if constexpr (WIDTH >= 16) v += dpp(v, std::integral_constant<int, 0x140>());  // the other half of a row (mirrored)
+    if constexpr (WIDTH == 32) {
+        const auto s = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+        v = __builtin_bit_cast(float, (unsigned)s[0]) + __builtin_bit_cast(float, (unsigned)s[1]);
+    }
     return v;
 }
 template <int WIDTH>

@@ -510,8 +510,8 @@ __global__ __launch_bounds__(256) void gemm_tn_join_kernel(const float* __restri
 
 struct Plan { int tile, tiles_m, tiles_n, splits, bias_splits; int64_t rows_split; };
 
-// 32-bit byte offsets within a workgroup's rows (and the eight stages that the loop may ask for behind them)
-bool offsets_fit(const Plan& p, int64_t ld_bytes) { return (p.rows_split + 8 * kBigBK) * ld_bytes < ((int64_t)1 << 31); }
+// 32-bit byte offsets within a workgroup's rows (and the stages that the loop asks for behind them, eight at most)
+bool offsets_fit(const Plan& p, int64_t ld_bytes) { return (p.rows_split + 16 * kBigBK) * ld_bytes < ((int64_t)1 << 31); }
 
 // tile 0: the narrow kernel (tiles of TM x TN)
 Plan plan(int64_t rows, int M, int N, int tile) {

@@ -30,46 +30,43 @@ template <bool E4M3, bool HAS_G, int D>
 struct PqOp {
     PqArgs a;
     static constexpr int LPR = D / 4;
-    struct Row { uint32_t q, scale; f32x4 g; };
-    struct Code { f32x4 e; };
-    __device__ __forceinline__ Row load(uint32_t row, int p, int col) const {
+    static constexpr bool kOwn = true;
+    // zn takes the place of the loads, g that of the output
+    struct Row { uint32_t q, scale; f32x4 g, e; };
+    __device__ __forceinline__ Row load(const equss::CodePair& at, int p, int col) const {
         Row r;
-        const int at = p * D + col;
-        r.q = *reinterpret_cast<const uint32_t*>(a.codes + (int64_t)row * a.ld_codes + at);
-        r.scale = a.scales[(int64_t)row * a.ld_scales + at / equss::kCkptBlock];
-        if constexpr (HAS_G) r.g = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(a.g_zq + (int64_t)row * a.ld_g + at));
+        const int c = p * D + col;
+        r.q = *reinterpret_cast<const uint32_t*>(a.codes + (int64_t)at.row * a.ld_codes + c);
+        r.scale = a.scales[(int64_t)at.row * a.ld_scales + c / equss::kCkptBlock];
+        r.g = f32x4{0.f, 0.f, 0.f, 0.f};
+        if constexpr (HAS_G) r.g = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(a.g_zq + (int64_t)at.row * a.ld_g + c));
+        r.e = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (at.code != a.K) r.e = *reinterpret_cast<const f32x4*>(a.books + ((int64_t)p * a.K + at.code) * D + col);
         return r;
     }
-    __device__ __forceinline__ Code code(int p, uint32_t k, int col) const {
-        Code c;
-        c.e = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (k != a.K) c.e = *reinterpret_cast<const f32x4*>(a.books + ((int64_t)p * a.K + k) * D + col);
-        return c;
-    }
-    __device__ __forceinline__ f32x4 value(const Row& r, const Code& c, uint32_t row, int p, int col, bool) const {
+    __device__ __forceinline__ f32x4 value(Row& r) const {
         const float s = a.g_vq[0] * a.inv_count, bs = a.beta * s;
         const f32x4 z = equss::ckpt_decode4<E4M3>(r.q) * equss::ckpt_scale(r.scale);
-        const float len = sqrtf(equss::group_sum<LPR>(z.x * z.x + z.y * z.y + z.z * z.z + z.w * z.w));
+        const float len = sqrtf(equss::lanes_sum<LPR>(z.x * z.x + z.y * z.y + z.z * z.z + z.w * z.w));
         const bool tiny = len < 1e-12f;
         const float inv = 1.f / (tiny ? 1e-12f : len);
         const f32x4 zn = z * inv;
-        if (a.g_z) {
-            f32x4 g;
+        f32x4 g;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) g[i] = fmaf(-bs, c.e[i], HAS_G ? r.g[i] : 0.f);
-            const float along = equss::group_sum<LPR>(zn.x * g.x + zn.y * g.y + zn.z * g.z + zn.w * g.w);
-            f32x4 o;
+        for (int i = 0; i < 4; ++i) g[i] = fmaf(-bs, r.e[i], r.g[i]);
+        const float along = equss::lanes_sum<LPR>(zn.x * g.x + zn.y * g.y + zn.z * g.z + zn.w * g.w);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = fmaf(zn[i], tiny ? bs : -along, g[i]) * inv;
-            __builtin_nontemporal_store(o, reinterpret_cast<f32x4*>(a.g_z + (int64_t)row * a.ld_gz + p * D + col));
-        }
-        return (zn - c.e) * (-a.book * s);
+        for (int i = 0; i < 4; ++i) r.g[i] = fmaf(zn[i], tiny ? bs : -along, g[i]) * inv;
+        return (zn - r.e) * (-a.book * s);
+    }
+    __device__ __forceinline__ void own(const Row& r, uint32_t row, int p, int col) const {
+        if (a.g_z) __builtin_nontemporal_store(r.g, reinterpret_cast<f32x4*>(a.g_z + (int64_t)row * a.ld_gz + p * D + col));
     }
 };
 
 template <int D>
 int run(const PqArgs& a, bool e4m3, const equss::SortPlan& s, const equss::IndexView& index, char* ws, float* g_books, hipStream_t st) {
-#define EQUSS_PQ(E, G) equss::walk_launch_lpr<PqOp<E, G, D>, D / 4>(PqOp<E, G, D>{a}, s, index, ws, g_books, D, a.g_z != nullptr, st)
+#define EQUSS_PQ(E, G) equss::walk_launch_lpr<PqOp<E, G, D>, D / 4>(PqOp<E, G, D>{a}, s, index, ws, g_books, D, st)
     if (e4m3) return a.g_zq ? EQUSS_PQ(true, true) : EQUSS_PQ(true, false);
     return a.g_zq ? EQUSS_PQ(false, true) : EQUSS_PQ(false, false);
 #undef EQUSS_PQ
