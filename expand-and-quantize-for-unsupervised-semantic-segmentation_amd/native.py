@@ -708,34 +708,54 @@ class ActCheckpoint:
         return ActCheckpoint(self.codes[:, start:last * CKPT_BLOCK], self.scales[:, start // CKPT_BLOCK:last], stop - start)
 
 
+def _kept(codes, scales, width):
+    """An ActCheckpoint of parts that are right by construction."""
+    ckpt = ActCheckpoint.__new__(ActCheckpoint)
+    ckpt.codes, ckpt.scales, ckpt.width = codes, scales, width
+    return ckpt
+
+
 def _row_major(t):
     """(t or a copy with unit column stride and rows that do not overlap, leading dimension)."""
     rows, width = t.shape
-    if (width > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < width):
-        t = t.contiguous()
-    return t, (t.stride(0) if rows > 1 else max(width, 1))
+    ld, unit = t.stride()
+    if (width > 1 and unit != 1) or (rows > 1 and ld < width):
+        return t.contiguous(), width
+    return t, (ld if rows > 1 else width)
 
 
 def _ckpt_parts(ckpt):
-    """Pointers and leading dimensions of a checkpoint in the layout the kernels take (column views included)."""
+    """Tensors and leading dimensions of a checkpoint in the layout the kernels take (column views included)."""
     codes, scales = ckpt.codes, ckpt.scales
-    if codes.shape[0] > 1 and (codes.stride(1) != 1 or codes.stride(0) % CKPT_BLOCK or codes.stride(0) < codes.shape[1]) or codes.data_ptr() % 16:
-        codes = codes.clone(memory_format=torch.contiguous_format)
+    rows, width = codes.shape
+    ld, unit = codes.stride()
+    if rows > 1 and (unit != 1 or ld % CKPT_BLOCK or ld < width) or codes.data_ptr() % 16:
+        codes, ld = codes.clone(memory_format=torch.contiguous_format), width
     scales, ld_scales = _row_major(scales)
-    return codes, (codes.stride(0) if codes.shape[0] > 1 else codes.shape[1]), scales, ld_scales
+    return codes, (ld if rows > 1 else width), scales, ld_scales
 
 
-def _same_device(*ts):
-    _need_cuda(*ts)
-    if len({t.device for t in ts if t is not None}) > 1:
-        raise ValueError("all tensors of a call must be on one device")
+def _same_device(first, *others):
+    if not first.is_cuda:
+        _need_cuda(first)
+    device = first.device
+    for t in others:
+        if t is not None and t.device != device:
+            _need_cuda(t)
+            raise ValueError("all tensors of a call must be on one device")
+
+
+def _at(t):
+    """A tensor's address for a call (None: NULL)."""
+    return t.data_ptr() if t is not None else None
 
 
 def ckpt_pack(x, fmt="int8", keep_sign=False):
     """x (rows, width) fp32 / bf16 / fp16 -> ActCheckpoint in ``fmt`` "int8" or "e4m3": one byte a value and one for 32
     consecutive channels.  ``keep_sign``: a value other than zero never becomes zero, so that ``code > 0`` is the mask of a
     ReLU whose result is kept (see equss_ckpt_pack in the header for the rounding)."""
-    _need_cuda(x)
+    if not x.is_cuda:
+        _need_cuda(x)
     if fmt not in CKPT_FORMATS:
         raise ValueError(f"Unsupported checkpoint format {fmt}")
     if x.dim() != 2 or x.dtype not in _ELEM_TYPES or x.shape[1] == 0:
@@ -743,11 +763,11 @@ def ckpt_pack(x, fmt="int8", keep_sign=False):
     x, ld = _row_major(x)
     rows, width = x.shape
     blocks = (width + CKPT_BLOCK - 1) // CKPT_BLOCK
-    codes = torch.empty((rows, blocks * CKPT_BLOCK), dtype=_CKPT_DTYPES[fmt], device=x.device)
-    scales = torch.empty((rows, blocks), dtype=torch.uint8, device=x.device)
-    _check(load_library().equss_ckpt_pack(_ptr(x), _ELEM_TYPES[x.dtype], ld, _ptr(codes), blocks * CKPT_BLOCK, _ptr(scales), blocks, rows,
+    codes = x.new_empty((rows, blocks * CKPT_BLOCK), dtype=_CKPT_DTYPES[fmt])
+    scales = x.new_empty((rows, blocks), dtype=torch.uint8)
+    _check(load_library().equss_ckpt_pack(_at(x), _ELEM_TYPES[x.dtype], ld, _at(codes), blocks * CKPT_BLOCK, _at(scales), blocks, rows,
                                           width, CKPT_FORMATS[fmt], int(bool(keep_sign)), _stream(x)), "equss_ckpt_pack")
-    return ActCheckpoint(codes, scales, width)
+    return _kept(codes, scales, width)
 
 
 def ckpt_unpack(ckpt, dtype=torch.float32):
@@ -756,8 +776,8 @@ def ckpt_unpack(ckpt, dtype=torch.float32):
     if dtype not in _ELEM_TYPES:
         raise ValueError("ckpt_unpack: dtype must be float32, bfloat16 or float16")
     codes, ld_codes, scales, ld_scales = _ckpt_parts(ckpt)
-    out = torch.empty((ckpt.rows, ckpt.width), dtype=dtype, device=codes.device)
-    _check(load_library().equss_ckpt_unpack(_ptr(codes), ld_codes, _ptr(scales), ld_scales, _ptr(out), _ELEM_TYPES[dtype], ckpt.width,
+    out = codes.new_empty((ckpt.rows, ckpt.width), dtype=dtype)
+    _check(load_library().equss_ckpt_unpack(_at(codes), ld_codes, _at(scales), ld_scales, _at(out), _ELEM_TYPES[dtype], ckpt.width,
                                             ckpt.rows, ckpt.width, CKPT_FORMATS[ckpt.fmt], _stream(codes)), "equss_ckpt_unpack")
     return out
 
@@ -775,14 +795,14 @@ def gemm_tn_ckpt(a, ckpt, relu=None, want_bias=False):
     a, lda = _row_major(a)
     codes, ld_codes, scales, ld_scales = _ckpt_parts(ckpt)
     mask, ld_mask = _ckpt_parts(relu)[:2] if relu is not None else (None, 0)
-    out = torch.empty((m, ckpt.width), dtype=torch.float32, device=a.device)
-    bias = torch.empty((m,), dtype=torch.float32, device=a.device) if want_bias else None
+    out = a.new_empty((m, ckpt.width), dtype=torch.float32)
+    bias = a.new_empty((m,), dtype=torch.float32) if want_bias else None
     lib = load_library()
     # (scratch is allocated for the call, not kept: a call captured into a graph then holds its own)
     nbytes = lib.equss_gemm_tn_ckpt_workspace_bytes(rows, m, ckpt.width)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=a.device) if nbytes else None
-    _check(lib.equss_gemm_tn_ckpt(_ptr(a), lda, _ptr(codes), ld_codes, _ptr(scales), ld_scales, CKPT_FORMATS[ckpt.fmt], _ptr(mask), ld_mask,
-                                  _ptr(out), ckpt.width, _ptr(bias), rows, m, ckpt.width, _ptr(ws), nbytes, _stream(a)),
+    ws = a.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _check(lib.equss_gemm_tn_ckpt(_at(a), lda, _at(codes), ld_codes, _at(scales), ld_scales, CKPT_FORMATS[ckpt.fmt], _at(mask), ld_mask,
+                                  _at(out), ckpt.width, _at(bias), rows, m, ckpt.width, _at(ws), nbytes, _stream(a)),
            "equss_gemm_tn_ckpt")
     return (out, bias) if want_bias else out
 
@@ -810,16 +830,17 @@ def pq_st_backward_ckpt(ckpt, books, idx, g_zq, g_vq, beta, book, want_rows=True
     if books.data_ptr() % 16:
         books = books.clone()
     idx = idx.contiguous()
-    g_vq = g_vq.reshape(1).float().contiguous()
-    dev = books.device
-    g_rows = torch.empty((n, num_pq * d), dtype=torch.float32, device=dev) if want_rows else None
-    g_books = torch.empty((num_pq, k, d), dtype=torch.float32, device=dev) if want_books else None
+    if g_vq.numel() != 1:
+        raise ValueError("pq_st_backward_ckpt: g_vq must hold one value")
+    g_vq = g_vq if g_vq.dtype == torch.float32 else g_vq.float()
+    g_rows = books.new_empty((n, num_pq * d)) if want_rows else None
+    g_books = books.new_empty((num_pq, k, d)) if want_books else None
     lib = load_library()
     nbytes = lib.equss_code_sums_sorted_workspace_bytes(n, num_pq, k, d)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _check(lib.equss_pq_st_backward_ckpt(_ptr(codes), ld_codes, _ptr(scales), ld_scales, CKPT_FORMATS[ckpt.fmt], _ptr(books), _ptr(idx),
-                                         _ptr(g_zq), (g_zq.stride(0) if n > 1 else num_pq * d) if g_zq is not None else 0, _ptr(g_vq),
-                                         float(beta), float(book), _ptr(g_rows), num_pq * d, _ptr(g_books), n, num_pq, k, d, _ptr(ws), nbytes,
+    ws = books.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _check(lib.equss_pq_st_backward_ckpt(_at(codes), ld_codes, _at(scales), ld_scales, CKPT_FORMATS[ckpt.fmt], _at(books), _at(idx),
+                                         _at(g_zq), (g_zq.stride(0) if n > 1 else num_pq * d) if g_zq is not None else 0, _at(g_vq),
+                                         float(beta), float(book), _at(g_rows), num_pq * d, _at(g_books), n, num_pq, k, d, _at(ws), nbytes,
                                          _stream(books)), "equss_pq_st_backward_ckpt")
     return g_rows, g_books
 
@@ -827,7 +848,7 @@ def pq_st_backward_ckpt(ckpt, books, idx, g_zq, g_vq, beta, book, want_rows=True
 def _index_args(idx, what):
     if idx.dim() != 2 or idx.dtype not in _INDEX_TYPES:
         raise ValueError(f"{what}: idx must be a (num_pq, rows) int64, int32 or int16 tensor")
-    return _ptr(idx), _INDEX_TYPES[idx.dtype], idx.stride(0), idx.stride(1)
+    return _at(idx), _INDEX_TYPES[idx.dtype], idx.stride(0), idx.stride(1)
 
 
 def code_lookup(idx, books, scale=1.0):
@@ -843,8 +864,8 @@ def code_lookup(idx, books, scale=1.0):
     books = books.contiguous()
     if books.data_ptr() % 16:
         books = books.clone()
-    out = torch.empty((rows, num_pq * d), dtype=books.dtype, device=books.device)
-    _check(load_library().equss_code_lookup(*where, _ptr(books), _ELEM_TYPES[books.dtype], float(scale), _ptr(out), num_pq * d, rows, num_pq,
+    out = books.new_empty((rows, num_pq * d), dtype=books.dtype)
+    _check(load_library().equss_code_lookup(*where, _at(books), _ELEM_TYPES[books.dtype], float(scale), _at(out), num_pq * d, rows, num_pq,
                                             k, d, _stream(books)), "equss_code_lookup")
     return out
 
@@ -859,12 +880,12 @@ def code_lookup_grad(g, idx, num_codes, scale=1.0):
         raise ValueError(f"code_lookup_grad: g must be a ({rows}, {num_pq}*d) float32, bfloat16 or float16 tensor")
     d = g.shape[1] // num_pq
     g, ld = _row_major(g)
-    out = torch.empty((num_pq, num_codes, d), dtype=torch.float32, device=g.device)
+    out = g.new_empty((num_pq, num_codes, d), dtype=torch.float32)
     lib = load_library()
     nbytes = lib.equss_code_sums_sorted_workspace_bytes(rows, num_pq, int(num_codes), d)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=g.device) if nbytes else None
-    _check(lib.equss_code_lookup_grad(_ptr(g), _ELEM_TYPES[g.dtype], ld, *where, float(scale), _ptr(out), rows, num_pq, int(num_codes), d,
-                                      _ptr(ws), nbytes, _stream(g)), "equss_code_lookup_grad")
+    ws = g.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _check(lib.equss_code_lookup_grad(_at(g), _ELEM_TYPES[g.dtype], ld, *where, float(scale), _at(out), rows, num_pq, int(num_codes), d,
+                                      _at(ws), nbytes, _stream(g)), "equss_code_lookup_grad")
     return out
 
 
