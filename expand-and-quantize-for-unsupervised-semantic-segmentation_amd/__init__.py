@@ -16,13 +16,13 @@ Reference class                                   -> here
 from . import configs, synth  # noqa: F401
 from . import dist_utils, native  # noqa: F401
 from .featurizer import DinoFeaturizer, VisionTransformer  # noqa: F401
-from .pqgo import DIONPQGO, Codebook, ProductQuantizerWrapper, STEGOLoss  # noqa: F401
+from .pqgo import DIONPQGO, Codebook, ProductQuantizerWrapper, STEGOLoss, code_lookup  # noqa: F401
 from .evaluator import UnSegEvaluator, ClusterLookup  # noqa: F401
 from .metric import UnSegMetrics  # noqa: F401
 from .wrapper import PQGOWrapper, build_model  # noqa: F401
 from . import quantizer  # noqa: F401
-from .index_dump import CodeIndexDump  # noqa: F401
+from .index_dump import CodeIndexDump, read_features  # noqa: F401
 
-__all__ = ["CodeIndexDump", "configs", "synth", "native", "dist_utils", "quantizer", "DinoFeaturizer", "VisionTransformer",
+__all__ = ["CodeIndexDump", "read_features", "code_lookup", "configs", "synth", "native", "dist_utils", "quantizer", "DinoFeaturizer", "VisionTransformer",
            "DIONPQGO", "Codebook", "ProductQuantizerWrapper", "STEGOLoss", "UnSegEvaluator", "ClusterLookup",
            "UnSegMetrics", "PQGOWrapper", "build_model"]

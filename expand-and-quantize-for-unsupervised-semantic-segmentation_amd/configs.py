@@ -26,13 +26,15 @@ _STEGO = dict(  # config/pqgo_baseline.yaml:68-122 (cocostuff27, vit-small)
 def pqgo_config(model_type="vit_small", patch_size=8, embed_dim=1024, num_pq=8, num_codebook=256,
                 num_classes=27, extra_classes=0, normalize="l2", need_initialized="uni",
                 pretrained_weights=None, output_type="vq0", drop_prob=0.1, beta=0.25, book=1.0,
-                jsd_temperature=0.1):
-    """A config/pqgo_baseline.yaml-shaped dictionary (only the keys the model path reads)."""
+                jsd_temperature=0.1, activation_checkpoint="none"):
+    """A config/pqgo_baseline.yaml-shaped dictionary (only the keys the model path reads).  activation_checkpoint is this
+    package's own key (``DIONPQGO.activation_checkpoint``); a configuration without it means "none"."""
     return deepcopy({
         "num_classes": num_classes,
         "dataset_name": "cocostuff27",
         "wandb": {"name": "PQGO_synthetic"},
         "model": {
+            "activation_checkpoint": activation_checkpoint,
             "pretrained": {
                 "model_type": model_type,
                 "dino_patch_size": patch_size,

@@ -12,7 +12,7 @@ import torch
 
 from . import native
 
-__all__ = ["CodeIndexDump"]
+__all__ = ["CodeIndexDump", "read_features"]
 
 _HEADER_BYTES = 128   # fixed-size .npy v1.0 header so the shape can be rewritten in place
 
@@ -101,3 +101,13 @@ class CodeIndexDump:
     def __exit__(self, *exc):
         self.close()
         return False
+
+
+@torch.no_grad()
+def read_features(prefix: str, quantizer, start: int = 0, stop: int = None, scale: float = 1.0) -> torch.Tensor:
+    """Rows [start, stop) of a dump turned back into quantised features: ``<prefix>_index.npy`` is memory-mapped, its int16 rows
+    go to the device as they are, and ``quantizer.lookup`` (a ProductQuantizerWrapper, on the device of its codebooks) gathers
+    their codewords.  Returns (rows, D) in the codebooks' type; indices the codebooks do not have give zeros."""
+    table = np.load(prefix + "_index.npy", mmap_mode="r")
+    rows = torch.from_numpy(np.ascontiguousarray(table[start:stop]))
+    return quantizer.lookup(rows.to(next(quantizer.parameters()).device), scale)

@@ -18,9 +18,16 @@ from . import native
 from .dist_utils import all_reduce_tensor
 from .featurizer import DinoFeaturizer
 
-__all__ = ["DIONPQGO", "Codebook", "ProductQuantizerWrapper", "STEGOLoss"]
+__all__ = ["DIONPQGO", "Codebook", "ProductQuantizerWrapper", "STEGOLoss", "code_lookup"]
 
 _PQ_DIMS = (16, 32, 64, 128)
+_KEEP = ("none",) + tuple(native.CKPT_FORMATS)     # what ``activation_checkpoint`` may say
+
+
+def _check_keep(value):
+    if value not in _KEEP:
+        raise ValueError(f"Unsupported activation checkpoint {value} (one of {', '.join(_KEEP)})")
+    return value
 
 
 # ------------------------------------------------------------------------------------------------
@@ -193,10 +200,15 @@ class _HeadFunction(torch.autograd.Function):
     accumulation on the HIP kernels (``native.gemm_tn_bf16`` for the weight gradients, ``native.gemm_bf16`` for the
     gradient through the second branch) -- the precision class of the reference's training pass, which runs these
     convolutions under fp16 autocast (train.py:80).  The frozen backbone needs no input gradient.
-    The HIP forward leaves [f | relu(W2a f + b2a)] behind in bf16, which is what the backward needs."""
+    The HIP forward leaves [f | relu(W2a f + b2a)] behind in bf16, which is what the backward needs.
+
+    ``keep`` "int8" / "e4m3": that pair is kept in 8 bits (``native.ckpt_pack``, signs kept, so that the ReLU's mask is exact)
+    and the weight gradients are taken straight from the codes, the mask and both biases' sums on the way
+    (``native.gemm_tn_ckpt``).  The biases then sum the bf16 rows that the products use too: one pass over the gradient less,
+    and each row's rounding (2^-9 of its value) is as often up as down."""
 
     @staticmethod
-    def forward(ctx, rows, w1, b1, w2a, b2a, w2b, b2b):
+    def forward(ctx, rows, w1, b1, w2a, b2a, w2b, b2b, keep="none"):
         n, c = rows.shape
         d = w1.shape[0]
         fh = torch.empty((n, 2 * c), dtype=torch.bfloat16, device=rows.device)
@@ -204,14 +216,34 @@ class _HeadFunction(torch.autograd.Function):
         w_cat = torch.cat((w1.reshape(d, c), w2b.reshape(d, c)), dim=1).to(torch.bfloat16).contiguous()
         code = native.expand_head(fh, w2a.reshape(c, c).to(torch.bfloat16).contiguous(), b2a.float().contiguous(),
                                   w_cat, (b1 + b2b).float().contiguous(), d)
-        ctx.save_for_backward(fh, w_cat)
+        ctx.kept = keep != "none"
+        if ctx.kept:
+            kept = native.ckpt_pack(fh, keep, keep_sign=True)
+            ctx.save_for_backward(kept.codes, kept.scales, w_cat)
+        else:
+            ctx.save_for_backward(fh, w_cat)
         ctx.shapes = (w1.shape, w2a.shape, w2b.shape)
         return code
 
     native_backward = True   # False: the same products as torch.mm calls (for comparisons)
 
     @staticmethod
+    def _backward_kept(ctx, g):
+        codes, scales, w_cat = ctx.saved_tensors
+        c = w_cat.shape[1] // 2
+        s1, s2a, s2b = ctx.shapes
+        kept = native.ActCheckpoint(codes, scales, 2 * c)
+        g_bf = g.to(torch.bfloat16)
+        dw_cat, db = native.gemm_tn_ckpt(g_bf, kept, want_bias=True)         # (D, 2C) = [dW1 | dW2b]
+        w2b_t = w_cat[:, c:].t().contiguous()
+        d_h = native.gemm_bf16(g_bf, w2b_t, None, native.EPI_BF16) if c % 128 == 0 and w_cat.shape[0] % 128 == 0 else torch.mm(g_bf, w2b_t.t())
+        dw2a, db2a = native.gemm_tn_ckpt(d_h, kept.columns(0, c), relu=kept.columns(c, 2 * c), want_bias=True)
+        return None, dw_cat[:, :c].reshape(s1), db, dw2a.reshape(s2a), db2a, dw_cat[:, c:].reshape(s2b), db, None
+
+    @staticmethod
     def backward(ctx, g):
+        if ctx.kept:
+            return _HeadFunction._backward_kept(ctx, g)
         fh, w_cat = ctx.saved_tensors
         c = fh.shape[1] // 2
         d = w_cat.shape[0]
@@ -228,7 +260,7 @@ class _HeadFunction(torch.autograd.Function):
             dw2a = torch.mm(d_pre.t(), fh[:, :c]).float()
         db = g.sum(0)
         return (None, dw_cat[:, :c].reshape(s1), db, dw2a.reshape(s2a), d_pre.float().sum(0),
-                dw_cat[:, c:].reshape(s2b), db)
+                dw_cat[:, c:].reshape(s2b), db, None)
 
 
 # ------------------------------------------------------------------------------------------------
@@ -264,15 +296,24 @@ class _PQStraightThrough(torch.autograd.Function):
     d z written once, d books by atomic adds) instead of autograd through ~15 elementwise ops on (rows, D) tensors:
         d zn   = g_zq + g_vq * 2 beta (zn - emb) / (n d P)          d z = (d zn - zn <zn, d zn>) / |z|
         d emb  = g_vq * 2 book (emb - zn) / (n d P)                  d books[p, k] = sum over rows with idx = k
-    Returns (zq rows, vq-loss, idx)."""
+    Returns (zq rows, vq-loss, idx).
+
+    ``keep`` "int8" / "e4m3": z is kept in 8 bits and emb not at all (the codebooks have it), 1.03 bytes a value instead of 8;
+    the gradients are the closed form's at the kept z, and the codebooks' are summed in a fixed order
+    (``native.pq_st_backward_ckpt``)."""
 
     @staticmethod
-    def forward(ctx, rows, books, beta, book):
+    def forward(ctx, rows, books, beta, book, keep="none"):
         num_pq, k, d = books.shape
         n = rows.shape[0]
         idx, emb, loss_sum = native.pq_assign(rows, books, "l2", False)
         vq = ((book + beta) * (loss_sum / float(n * d))).mean()
-        ctx.save_for_backward(rows, emb, idx)
+        ctx.kept = keep != "none"
+        if ctx.kept:
+            kept = native.ckpt_pack(rows, keep)
+            ctx.save_for_backward(kept.codes, kept.scales, books, idx)
+        else:
+            ctx.save_for_backward(rows, emb, idx)
         ctx.meta = (num_pq, k, d, float(beta), float(book))
         ctx.mark_non_differentiable(idx)
         return emb, vq, idx
@@ -281,15 +322,22 @@ class _PQStraightThrough(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g_zq, g_vq, _g_idx):
-        rows, emb, idx = ctx.saved_tensors
         num_pq, k, d, beta, book = ctx.meta
+        if ctx.kept:
+            codes, scales, books, idx = ctx.saved_tensors
+            if g_vq is None:
+                g_vq = torch.zeros((), dtype=torch.float32, device=codes.device)
+            g_rows, g_books = native.pq_st_backward_ckpt(native.ActCheckpoint(codes, scales, num_pq * d), books, idx, g_zq, g_vq, beta, book,
+                                                         want_rows=ctx.needs_input_grad[0], want_books=ctx.needs_input_grad[1])
+            return g_rows, g_books, None, None, None
+        rows, emb, idx = ctx.saved_tensors
         n = rows.shape[0]
         if _PQStraightThrough.hip_backward:
             if g_vq is None:
                 g_vq = torch.zeros((), dtype=torch.float32, device=rows.device)
             g_rows, g_books = native.pq_st_backward(rows, emb, idx, g_zq, g_vq, beta, book, k, d,
                                                     want_rows=ctx.needs_input_grad[0], want_books=ctx.needs_input_grad[1])
-            return g_rows, g_books, None, None
+            return g_rows, g_books, None, None, None
         z3 = rows.reshape(n, num_pq, d)
         norm = z3.norm(dim=-1, keepdim=True).clamp_min(1e-12)     # F.normalize's eps
         zn = z3 / norm
@@ -308,13 +356,35 @@ class _PQStraightThrough(torch.autograd.Function):
                 g_zn += g_zq.reshape(n, num_pq, d)
             proj = (zn * g_zn).sum(dim=-1, keepdim=True)
             g_rows = (g_zn.addcmul_(zn, proj, value=-1.0) / norm).reshape(n, num_pq * d)
-        return g_rows, g_books, None, None
+        return g_rows, g_books, None, None, None
+
+
+class _CodeLookup(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, idx, books, scale):
+        ctx.save_for_backward(idx)
+        ctx.meta = (books.shape[1], scale, books.dtype)
+        return native.code_lookup(idx, books, scale)
+
+    @staticmethod
+    def backward(ctx, g):
+        (idx,) = ctx.saved_tensors
+        k, scale, dtype = ctx.meta
+        return None, native.code_lookup_grad(g, idx, k, scale).to(dtype), None
+
+
+def code_lookup(idx, books, scale=1.0):
+    """Codewords by their indices (the gather of dino_pqgo.py:659-663 on its own): idx (num_pq, rows) integer, any strides; books
+    (num_pq, K, d) -> (rows, num_pq*d) = scale * books[p, idx[p, r]], zeros where an index lies outside [0, K).  Differentiable
+    in the books; the gradient sums every codeword's rows in a fixed order."""
+    return _CodeLookup.apply(idx, books, float(scale))
 
 
 def _quantize_rows(rows, books, normalize, beta, book, training, vq_counts, gather_normalized=False,
-                   use_restart=False, quantizers=None):
+                   use_restart=False, quantizers=None, keep="none"):
     """Shared core of Codebook / ProductQuantizerWrapper.
-    rows (n, num_pq*d) fp32, books (num_pq, K, d).  Returns zq rows, idx (num_pq, n), output dict."""
+    rows (n, num_pq*d) fp32, books (num_pq, K, d).  Returns zq rows, idx (num_pq, n), output dict.
+    keep: what the l2 training branch saves z in for its backward, "none" (fp32), "int8" or "e4m3"."""
     num_pq, k, d = books.shape
     n = rows.shape[0]
     output = {}
@@ -323,7 +393,9 @@ def _quantize_rows(rows, books, normalize, beta, book, training, vq_counts, gath
         per_pq = loss_sum / float(n * d)                       # mse per sub-space
         output["vq-loss"] = ((book + beta) * per_pq).mean()    # dino_pqgo.py:685-687 then :771-772
     elif normalize == "l2" and not gather_normalized and rows.is_cuda:
-        zq, vq, idx = _PQStraightThrough.apply(rows, books, beta, book)
+        if keep != "none" and use_restart:
+            books = books.clone()     # (the backward reads them, and a restart below writes the parameter they may be a view of)
+        zq, vq, idx = _PQStraightThrough.apply(rows, books, beta, book, keep)
         output["vq-loss"] = vq
     else:
         idx, _, _ = native.pq_assign(rows.detach(), books.detach(), normalize, gather_normalized,
@@ -334,7 +406,7 @@ def _quantize_rows(rows, books, normalize, beta, book, training, vq_counts, gath
         z3 = rows.reshape(n, num_pq, d)
         zn, cn = _torch_normalize(z3, books, normalize)
         table = cn if gather_normalized else books
-        emb = torch.gather(table, 1, idx.unsqueeze(-1).expand(num_pq, n, d)).permute(1, 0, 2)   # (n, num_pq, d)
+        emb = code_lookup(idx, table).reshape(n, num_pq, d)
         cb_loss = ((emb - zn.detach()) ** 2).mean(dim=(0, 2))
         commit = ((zn - emb.detach()) ** 2).mean(dim=(0, 2))
         output["vq-loss"] = (book * cb_loss + beta * commit).mean()
@@ -397,6 +469,8 @@ class Codebook(nn.Module):
         self.use_restart, self.use_split = use_restart, use_split
         self.need_initialized = need_initialized
         self.jsd_ts = jsd_ts
+        # what the training pass keeps its input in for the backward: "none" (fp32), "int8" or "e4m3" (l2 normalisation only)
+        self.activation_checkpoint = "none"
 
     @torch.no_grad()
     def prepare_restart(self, vq_current_count: torch.Tensor, z_flat: torch.Tensor) -> None:
@@ -443,6 +517,11 @@ class Codebook(nn.Module):
             nn.init.xavier_normal_(self.embedding.weight)
         self.need_initialized = "none"
 
+    def lookup(self, index: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+        """Codewords by their indices, as forward's fourth result has them: (b, h, w) integer -> (b, d, h, w); see code_lookup."""
+        b, h, w = index.shape
+        return _nchw_of(code_lookup(index.reshape(1, -1), self.embedding.weight.unsqueeze(0), scale), b, h, w)
+
     def forward(self, z: torch.Tensor, z_pos: torch.Tensor = None, return_prob: bool = True):
         """(b, d, h, w) -> (z_q (b,d,h,w), {"vq-loss"[, "codebook-usage"]}, distance_prob (b,h,w,K), idx (b,h,w)).
         z_pos is accepted for signature parity; nothing the reference returns depends on it."""
@@ -455,7 +534,8 @@ class Codebook(nn.Module):
             self.initialize_from(rows.detach())
         books = self.embedding.weight.unsqueeze(0)
         zq, idx, output = _quantize_rows(rows, books, self.normalize, self.beta, self.book, self.training,
-                                         None, use_restart=self.use_restart, quantizers=[self])
+                                         None, use_restart=self.use_restart, quantizers=[self],
+                                         keep=_check_keep(self.activation_checkpoint))
         prob = None
         if return_prob:
             prob = native.pq_prob(rows.detach(), books.detach(), self.normalize, self.jsd_ts).reshape(b, h, w, -1)
@@ -483,6 +563,21 @@ class ProductQuantizerWrapper(nn.Module):
             for _ in range(self.num_pq)])
         self._books = None
         self._books_key = None
+        # what the training pass keeps its input in for the backward: "none" (fp32), "int8" or "e4m3" (l2 normalisation only)
+        self.activation_checkpoint = "none"
+
+    def lookup(self, z_index: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+        """The features that indices stand for.  (num_pq, b, h, w) integer, as DIONPQGO.forward stacks them -> (b, D, h, w);
+        (rows, num_pq) integer, as CodeIndexDump stores them -> (rows, D).  See code_lookup."""
+        books = self.stacked_codebooks()
+        if z_index.dim() == 2:
+            if z_index.shape[1] != self.num_pq:
+                raise ValueError(f"expected rows of {self.num_pq} indices, got {z_index.shape[1]}")
+            return code_lookup(z_index.t(), books, scale)
+        if z_index.dim() != 4 or z_index.shape[0] != self.num_pq:
+            raise ValueError(f"expected ({self.num_pq}, b, h, w) or (rows, {self.num_pq}) indices, got {tuple(z_index.shape)}")
+        _, b, h, w = z_index.shape
+        return _nchw_of(code_lookup(z_index.reshape(self.num_pq, -1), books, scale), b, h, w)
 
     def stacked_codebooks(self) -> torch.Tensor:
         """(num_pq, K, d) view of all sub-codebooks.  In training the stack is rebuilt (differentiable);
@@ -519,7 +614,8 @@ class ProductQuantizerWrapper(nn.Module):
                     q.initialize_from(rows.detach()[:, i * self.pq_dim:(i + 1) * self.pq_dim])
         books = self.stacked_codebooks()
         zq, idx, outputs = _quantize_rows(rows, books, q0.normalize, q0.beta, q0.book, self.training, None,
-                                          use_restart=q0.use_restart, quantizers=self.quantizers)
+                                          use_restart=q0.use_restart, quantizers=self.quantizers,
+                                          keep=_check_keep(self.activation_checkpoint))
         z_q = _nchw_of(zq, b, h, w)
         z_split = torch.chunk(z, chunks=self.num_pq, dim=1)
         z_quantized = list(torch.chunk(z_q, chunks=self.num_pq, dim=1))
@@ -581,6 +677,7 @@ class DIONPQGO(nn.Module):
         else:
             raise ValueError(f"Unsupported vq type {self.vq_type}.")
         self.stego_loss = STEGOLoss(cfg=self.cfg_loss["stego"])
+        self.activation_checkpoint = cfg.get("activation_checkpoint", "none")
         self._head = None
         self._head_key = None
         # eval forward: image ranges of a batch run on this many HIP streams (1 = everything on the caller's)
@@ -610,7 +707,8 @@ class DIONPQGO(nn.Module):
         view of token-major memory); see _HeadFunction."""
         b, c, h, w = feat.shape
         w1, w2a, w2b = self.cluster1[0], self.cluster2[0], self.cluster2[2]
-        code = _HeadFunction.apply(_rows_of(feat), w1.weight, w1.bias, w2a.weight, w2a.bias, w2b.weight, w2b.bias)
+        code = _HeadFunction.apply(_rows_of(feat), w1.weight, w1.bias, w2a.weight, w2a.bias, w2b.weight, w2b.bias,
+                                   self.activation_checkpoint)
         return _nchw_of(code, b, h, w)
 
     def _head_weights(self):
@@ -625,6 +723,19 @@ class DIONPQGO(nn.Module):
                               w_cat=w_cat.to(torch.bfloat16).contiguous(), b_cat=(b1 + b2b).contiguous())
             self._head_key = key
         return self._head
+
+    @property
+    def activation_checkpoint(self) -> str:
+        """What a training step keeps of the head's inputs and of the quantiser's between forward and backward: "none" (default:
+        bf16 and fp32), or 8-bit checkpoints "int8" / "e4m3" with a scale for 32 channels (``native.ckpt_pack``): about a quarter
+        of the bytes, weight gradients off by the rounding of what was kept (a block's largest value has 7 / 4 bits)."""
+        return self._activation_checkpoint
+
+    @activation_checkpoint.setter
+    def activation_checkpoint(self, value: str) -> None:
+        self._activation_checkpoint = _check_keep(value)
+        for blk in self.vq_blocks:
+            blk.activation_checkpoint = value
 
     @property
     def precision(self) -> str:

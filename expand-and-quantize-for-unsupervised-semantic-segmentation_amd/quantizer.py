@@ -12,6 +12,7 @@ import torch.nn.functional as F
 
 from . import native
 from .dist_utils import all_reduce_tensor
+from .pqgo import code_lookup
 
 __all__ = ["VectorQuantizer", "EMAVectorQuantizer", "EmbeddingEMA", "ProductQuantizerWrapper",
            "get_histogram_count"]
@@ -128,7 +129,7 @@ class VectorQuantizer(_RestartMixin, nn.Module):
         else:
             idx, _, _ = native.pq_assign(rows.detach(), books.detach(), mode, True, want_zq=False, want_loss=False)
             zn, cn = _torch_norm(rows, self.codebook.weight, mode)
-            emb = F.embedding(idx[0], cn)
+            emb = code_lookup(idx, cn.unsqueeze(0))
             codebook_loss = F.mse_loss(emb, zn.detach())
             commitment_loss = F.mse_loss(zn, emb.detach())
             zq = zn + (emb - zn).detach()

@@ -26,6 +26,8 @@ def main():
     ap.add_argument("--res", type=int, default=224)
     ap.add_argument("--steps", type=int, default=10)
     ap.add_argument("--warmup", type=int, default=3)
+    ap.add_argument("--keep", choices=("none", "int8", "e4m3"), default="none",
+                    help="what the step keeps of its activations between forward and backward")
     args = ap.parse_args()
     rank = int(os.environ.get("RANK", "0"))
     local_rank = int(os.environ.get("LOCAL_RANK", "0"))
@@ -39,7 +41,7 @@ def main():
         os.environ.setdefault("MASTER_ADDR", "127.0.0.1")
         dist.init_process_group(backend="nccl")
     pkg = importlib.import_module(PKG)
-    cfg = pkg.configs.pqgo_config(need_initialized="uni")
+    cfg = pkg.configs.pqgo_config(need_initialized="uni", activation_checkpoint=args.keep)
     wrapper = pkg.build_model(cfg)
     wrapper.load_state_dict(pkg.synth.synth_pqgo_state(cfg, seed=1234), strict=True)
     wrapper = wrapper.to(dev).train()
@@ -63,6 +65,7 @@ def main():
     for i in range(args.warmup):
         step(i)
     torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats(dev)
     if dist is not None:
         dist.barrier()
     t0 = time.perf_counter()
@@ -81,6 +84,7 @@ def main():
                                       f"{args.batch} x {args.res}^2 per GPU (+ positive pair), synthetic",
                           "n_gpus": world, "images_per_s": round(world * args.batch * args.steps / dt, 1),
                           "ms_per_step": round(dt / args.steps * 1e3, 2),
+                          "keep": args.keep, "peak_memory_gb": round(torch.cuda.max_memory_allocated(dev) / 1e9, 3),
                           "losses": {k: round(float(torch.as_tensor(v).detach()), 5) for k, v in out.items() if k != "end_time"}}))
     if dist is not None:
         dist.destroy_process_group()
