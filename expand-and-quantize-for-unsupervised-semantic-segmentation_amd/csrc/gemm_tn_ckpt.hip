@@ -494,15 +494,13 @@ __global__ __launch_bounds__(256) void gemm_tn_join_kernel(const float* __restri
         const int64_t step = main ? split_c : split_bias;
         const int n = main ? splits : bias_splits;
         float s = 0.f;
-        int k = 0;
-        for (; k + 8 <= n; k += 8) {
-            float v[8];
+        for (int k = 0; k < n; k += 16) {                  // (sixteen loads in flight: one row range is a load, and they add up)
+            float v[16];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = p[(k + j) * step];
+            for (int j = 0; j < 16; ++j) v[j] = p[(k + j < n ? k + j : n - 1) * step];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s += v[j];
+            for (int j = 0; j < 16; ++j) s += k + j < n ? v[j] : 0.f;
         }
-        for (; k < n; ++k) s += p[k * step];
         if (main) c[(i / N) * ldc + i % N] = s;
         else bias[i - cells] = s;
     }
@@ -521,12 +519,16 @@ Plan plan(int64_t rows, int M, int N, int tile) {
     p.tiles_m = (M + t - 1) / t;
     p.tiles_n = (N + t - 1) / t;
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-    // Row ranges: one more shortens everybody's loop (0.4 us for 32 rows) and adds a partial product to write and read back
-    // (8 M N bytes at 5 TB/s); the sum is least near splits^2 = 7800 rows / (M N).  At most one round of workgroups.
+    // Row ranges: more of them shorten everybody's loop (32 rows take 0.35 us, 0.75 us with the large tile and all CUs at work),
+    // but two or more need the join (6 us for its launch and what it waits for), and each writes and reads back a partial product
+    // (0.08 us + 1.1 us for a million elements).  The cheapest number, at most one round of workgroups.
+    const int64_t most = (tile == 256 ? 256 : 512) / tiles, steps = (rows + bk - 1) / bk;
     int64_t splits = 1;
-    const int64_t most = (tile == 256 ? 256 : 512) / tiles, steps = (rows + 4 * bk - 1) / (4 * bk);   // at least four steps a workgroup
-    while (splits < most && splits < steps && (splits + 1) * (splits + 1) * (double)M * N <= 7800.0 * (double)rows) ++splits;
-    if (splits < 1) splits = 1;
+    double best = 1e300;
+    for (int64_t s = 1; s <= (most > 1 ? most : 1) && (s == 1 || 4 * s <= steps); ++s) {   // at least four steps a workgroup
+        const double cost = (double)((steps + s - 1) / s) * (tile == 256 ? 0.75 : 0.35) + (s > 1 ? 6.0 + (double)s * (0.08 + 1.1e-6 * M * N) : 0.0);
+        if (cost < best) { best = cost; splits = s; }
+    }
     p.rows_split = ((rows + splits - 1) / splits + bk - 1) / bk * bk;
     if (p.rows_split < bk) p.rows_split = bk;
     p.splits = (int)((rows + p.rows_split - 1) / p.rows_split);
