@@ -122,15 +122,18 @@ struct GradOp {
     int d;
     typedef f32x4 Row;
     static constexpr bool kOwn = false;
+    template <bool ONCE>
     __device__ __forceinline__ Row load(const equss::CodePair& at, int p, int col) const {
         const typename Elem<T>::type* s = g + (int64_t)at.row * ld + (int64_t)p * d + col;
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
         if (col + 4 <= d) {
             if constexpr (T == 0) {
-                const f32x4u w = *reinterpret_cast<const f32x4u*>(s);
+                const f32x4u* from = reinterpret_cast<const f32x4u*>(s);
+                const f32x4u w = ONCE ? __builtin_nontemporal_load(from) : *from;
                 v = f32x4{w[0], w[1], w[2], w[3]};
             } else {
-                const u32x2u2 w = *reinterpret_cast<const u32x2u2*>(s);
+                const u32x2u2* from = reinterpret_cast<const u32x2u2*>(s);
+                const u32x2u2 w = ONCE ? __builtin_nontemporal_load(from) : *from;
                 if constexpr (T == 1) {
                     v = f32x4{equss::bits_as<float>(w[0] << 16), equss::bits_as<float>(w[0] & 0xffff0000u),
                               equss::bits_as<float>(w[1] << 16), equss::bits_as<float>(w[1] & 0xffff0000u)};
@@ -147,6 +150,7 @@ struct GradOp {
         return v;
     }
     __device__ __forceinline__ f32x4 value(Row& r) const { return r * scale; }
+    template <bool ONCE>
     __device__ __forceinline__ void own(const Row&, uint32_t, int, int) const {}
 };
 

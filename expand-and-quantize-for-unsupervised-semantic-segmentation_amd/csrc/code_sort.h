@@ -83,9 +83,10 @@ int sort_launch(const SortPlan& s, const IndexView& index, char* ws, size_t* pai
 // --------------------------------------------------------------------------------------------------------------------------
 // The walk.  Op gives the kernels their rows:
 //   struct Row;                             what is loaded of one (code, row) pair and lane
-//   Row  load(pair, p, col) const           its loads
+//   Row  load<ONCE>(pair, p, col) const     its loads; ONCE: more data than the caches hold, past them where a row is not shared
 //   f32x4 value(const Row&) const           the lane's four terms of the sum
-//   kOwn; void own(const Row&, row, p, col) whether there is one, and the row's own output, if it has one; after value(), which may keep what it needs in Row
+//   kOwn; own<ONCE>(const Row&, row, p, col)   whether a row has an output of its own, and its store; after value(), which may
+//                                           leave what it needs in Row
 // A row's part of d elements is walked by LPR lanes with four elements each (d <= 4 LPR; beyond 256 in chunks of 256 columns).
 
 struct WalkArgs {
@@ -108,7 +109,8 @@ __device__ __forceinline__ void store_cols(float* p, f32x4 v, int col, int d, bo
 }
 
 // U: pairs in flight a group.  One where the chip is full of groups (102400 rows, 8 x 256 x 128, the quantiser's backward: 223 us
-// with 1, 251 with 2, 267 with 4), two where it is not (4096 rows: 33 / 30 / 31 us).
+// with 1, 251 with 2, 267 with 4), two where it is not (4096 rows: 33 / 30 / 31 us).  The rows of the first kind go past the
+// caches (lookup gradient of 102400 rows: 99 us, 110 us through them; of 16384 rows: 33 / 32 us).
 template <class Op, int LPR, int U>
 __global__ __launch_bounds__(256) void code_accumulate_kernel(const Op op, const WalkArgs w) {
     constexpr int SLOTS = 64 / LPR;
@@ -135,7 +137,7 @@ __global__ __launch_bounds__(256) void code_accumulate_kernel(const Op op, const
 #pragma unroll
         for (int j = 0; j < U; ++j) {
             pr[j] = next[j];
-            row[j] = op.load(pr[j], p, live ? col : 0);
+            row[j] = op.template load<U == 1>(pr[j], p, live ? col : 0);
         }
 #pragma unroll
         for (int j = 0; j < U; ++j) next[j] = pairs[i + U + j < t1 ? i + U + j : t1 - 1];
@@ -143,7 +145,7 @@ __global__ __launch_bounds__(256) void code_accumulate_kernel(const Op op, const
 #pragma unroll
         for (int j = 0; j < U; ++j) v[j] = op.value(row[j]);
 #pragma unroll
-        for (int j = 0; j < U; ++j) op.own(row[j], pr[j].row, p, col);
+        for (int j = 0; j < U; ++j) op.template own<U == 1>(row[j], pr[j].row, p, col);
 #pragma unroll
         for (int j = 0; j < U; ++j) {
             if (i + j < t1) {
@@ -277,14 +279,14 @@ __global__ __launch_bounds__(256) void code_small_kernel(const Op op, const Inde
             typename Op::Row row[4];
             f32x4 v[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) row[i] = op.load(list[j + i < hi ? j + i : hi - 1], p, live ? col : 0);
+            for (int i = 0; i < 4; ++i) row[i] = op.template load<false>(list[j + i < hi ? j + i : hi - 1], p, live ? col : 0);
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] = op.value(row[i]);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (j + i < hi) {
                     acc += v[i];
-                    op.own(row[i], list[j + i].row, p, col);
+                    op.template own<false>(row[i], list[j + i].row, p, col);
                 }
         }
         return acc;
@@ -355,13 +357,13 @@ __global__ __launch_bounds__(256) void code_small_kernel(const Op op, const Inde
             if (!any) continue;
             typename Op::Row row[FLIGHT];
 #pragma unroll
-            for (int i = 0; i < FLIGHT; ++i) row[i] = op.load(pr[i], p, live ? col : 0);
+            for (int i = 0; i < FLIGHT; ++i) row[i] = op.template load<false>(pr[i], p, live ? col : 0);
 #pragma unroll
             for (int i = 0; i < FLIGHT; ++i) {
                 const f32x4 v = op.value(row[i]);
                 if (j + i < hi && pr[i].code == k) {
                     acc += v;
-                    op.own(row[i], pr[i].row, p, col);
+                    op.template own<false>(row[i], pr[i].row, p, col);
                 }
             }
         }

@@ -33,13 +33,17 @@ struct PqOp {
     static constexpr bool kOwn = true;
     // zn takes the place of the loads, g that of the output
     struct Row { uint32_t q, scale; f32x4 g, e; };
+    template <bool ONCE>
     __device__ __forceinline__ Row load(const equss::CodePair& at, int p, int col) const {
         Row r;
         const int c = p * D + col;
         r.q = *reinterpret_cast<const uint32_t*>(a.codes + (int64_t)at.row * a.ld_codes + c);
         r.scale = a.scales[(int64_t)at.row * a.ld_scales + c / equss::kCkptBlock];
         r.g = f32x4{0.f, 0.f, 0.f, 0.f};
-        if constexpr (HAS_G) r.g = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(a.g_zq + (int64_t)at.row * a.ld_g + c));
+        if constexpr (HAS_G) {
+            const f32x4* from = reinterpret_cast<const f32x4*>(a.g_zq + (int64_t)at.row * a.ld_g + c);
+            r.g = ONCE ? __builtin_nontemporal_load(from) : *from;
+        }
         r.e = f32x4{0.f, 0.f, 0.f, 0.f};
         if (at.code != a.K) r.e = *reinterpret_cast<const f32x4*>(a.books + ((int64_t)p * a.K + at.code) * D + col);
         return r;
@@ -59,8 +63,12 @@ struct PqOp {
         for (int i = 0; i < 4; ++i) r.g[i] = fmaf(zn[i], tiny ? bs : -along, g[i]) * inv;
         return (zn - r.e) * (-a.book * s);
     }
+    template <bool ONCE>
     __device__ __forceinline__ void own(const Row& r, uint32_t row, int p, int col) const {
-        if (a.g_z) __builtin_nontemporal_store(r.g, reinterpret_cast<f32x4*>(a.g_z + (int64_t)row * a.ld_gz + p * D + col));
+        if (!a.g_z) return;
+        f32x4* to = reinterpret_cast<f32x4*>(a.g_z + (int64_t)row * a.ld_gz + p * D + col);
+        if constexpr (ONCE) __builtin_nontemporal_store(r.g, to);
+        else *to = r.g;
     }
 };
 
