@@ -316,6 +316,7 @@ class _PQStraightThrough(torch.autograd.Function):
             ctx.save_for_backward(rows, emb, idx)
         ctx.meta = (num_pq, k, d, float(beta), float(book))
         ctx.mark_non_differentiable(idx)
+        ctx.set_materialize_grads(False)      # no (n, D) tensor of zeros where nothing comes back through zq
         return emb, vq, idx
 
     hip_backward = True   # False: the closed form below with stock elementwise ops and index_add_ (for comparisons)
