@@ -159,7 +159,7 @@ int index_checks(const char* what, const void* idx, int index_type, int64_t rows
         return equss::fail(EQUSS_E_SHAPE, "%s: rows=%lld num_pq=%d K=%lld d=%d", what, (long long)rows, num_pq, (long long)K, d);
     if (index_type < EQUSS_I64 || index_type > EQUSS_I16 || type < EQUSS_F32 || type > EQUSS_F16)
         return equss::fail(EQUSS_E_UNSUPPORTED, "%s: index type %d, element type %d", what, index_type, type);
-    if (num_pq > 65535 || (int64_t)num_pq * d > (1 << 24) || K >= ((int64_t)1 << 31) || rows > 0x7fffff00)
+    if (num_pq > 65535 || d > (1 << 23) || (int64_t)num_pq * d > (1 << 24) || K >= ((int64_t)1 << 31) || rows > 0x7fffff00)
         return equss::fail(EQUSS_E_UNSUPPORTED, "%s: rows=%lld num_pq=%d K=%lld d=%d", what, (long long)rows, num_pq, (long long)K, d);
     if (rows > 0 && !idx) return equss::fail(EQUSS_E_NULL, "%s: null pointer argument", what);
     return EQUSS_OK;

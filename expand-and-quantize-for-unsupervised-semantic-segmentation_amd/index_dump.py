@@ -109,5 +109,5 @@ def read_features(prefix: str, quantizer, start: int = 0, stop: int = None, scal
     go to the device as they are, and ``quantizer.lookup`` (a ProductQuantizerWrapper, on the device of its codebooks) gathers
     their codewords.  Returns (rows, D) in the codebooks' type; indices the codebooks do not have give zeros."""
     table = np.load(prefix + "_index.npy", mmap_mode="r")
-    rows = torch.from_numpy(np.ascontiguousarray(table[start:stop]))
+    rows = torch.from_numpy(np.array(table[start:stop]))
     return quantizer.lookup(rows.to(next(quantizer.parameters()).device), scale)

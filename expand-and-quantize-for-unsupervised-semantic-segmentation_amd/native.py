@@ -729,7 +729,7 @@ def _ckpt_parts(ckpt):
     codes, scales = ckpt.codes, ckpt.scales
     rows, width = codes.shape
     ld, unit = codes.stride()
-    if rows > 1 and (unit != 1 or ld % CKPT_BLOCK or ld < width) or codes.data_ptr() % 16:
+    if unit != 1 or (rows > 1 and (ld % CKPT_BLOCK or ld < width)) or codes.data_ptr() % 16:
         codes, ld = codes.clone(memory_format=torch.contiguous_format), width
     scales, ld_scales = _row_major(scales)
     return codes, (ld if rows > 1 else width), scales, ld_scales
@@ -878,6 +878,8 @@ def code_lookup_grad(g, idx, num_codes, scale=1.0):
     num_pq, rows = idx.shape
     if g.dim() != 2 or g.dtype not in _ELEM_TYPES or g.shape[0] != rows or num_pq == 0 or g.shape[1] == 0 or g.shape[1] % num_pq:
         raise ValueError(f"code_lookup_grad: g must be a ({rows}, {num_pq}*d) float32, bfloat16 or float16 tensor")
+    if num_codes <= 0:
+        raise ValueError(f"code_lookup_grad: {num_codes} codes")
     d = g.shape[1] // num_pq
     g, ld = _row_major(g)
     out = g.new_empty((num_pq, num_codes, d), dtype=torch.float32)

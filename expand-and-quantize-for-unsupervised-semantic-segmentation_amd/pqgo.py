@@ -361,6 +361,9 @@ class _PQStraightThrough(torch.autograd.Function):
 
 
 class _CodeLookup(torch.autograd.Function):
+    """out = scale * books[p, idx[p, r]]; linear in the books, and so is its gradient in its own input: each is the other's
+    backward, to any order."""
+
     @staticmethod
     def forward(ctx, idx, books, scale):
         ctx.save_for_backward(idx)
@@ -371,7 +374,21 @@ class _CodeLookup(torch.autograd.Function):
     def backward(ctx, g):
         (idx,) = ctx.saved_tensors
         k, scale, dtype = ctx.meta
-        return None, native.code_lookup_grad(g, idx, k, scale).to(dtype), None
+        return None, _CodeLookupGrad.apply(idx, g, k, scale).to(dtype), None
+
+
+class _CodeLookupGrad(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, idx, g, k, scale):
+        ctx.save_for_backward(idx)
+        ctx.meta = (scale, g.dtype)
+        return native.code_lookup_grad(g, idx, k, scale)
+
+    @staticmethod
+    def backward(ctx, gg):
+        (idx,) = ctx.saved_tensors
+        scale, dtype = ctx.meta
+        return None, _CodeLookup.apply(idx, gg, scale).to(dtype), None, None
 
 
 def code_lookup(idx, books, scale=1.0):

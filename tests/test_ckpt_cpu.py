@@ -75,7 +75,7 @@ def test_lookup_and_its_gradient_check_their_arguments(native):
 
     assert look(idx=None) == look(books=None) == look(out=None) == NULL
     assert look(rows=-1) == look(num_pq=0) == look(k=0) == look(d=0) == SHAPE
-    assert look(it=3) == look(type=3) == look(k=1 << 31) == look(rows=(1 << 31) - 1) == look(num_pq=70000, ld_out=70000 * 16) == UNSUPPORTED
+    assert look(it=3) == look(type=3) == look(k=1 << 31) == look(rows=(1 << 31) - 1) == look(num_pq=70000, ld_out=70000 * 16) == look(num_pq=1, d=1 << 24, ld_out=1 << 24) == UNSUPPORTED
     assert look(ld_out=63) == look(books=ctypes.c_void_p((1 << 20) + 4)) == look(out=ctypes.c_void_p((1 << 20) + 2)) == ALIGN
     assert look(rows=0, idx=None, books=None, out=None) == 0
 

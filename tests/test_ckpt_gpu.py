@@ -186,8 +186,13 @@ def test_weight_gradient_takes_views_and_no_rows(native, dev):
     # a block of NaN spoils its own columns only
     x = torch.randn(64, 96, device=dev)
     x[10, 40] = float("inf")
-    dw = native.gemm_tn_ckpt(big[:64], native.ckpt_pack(x))
-    assert bool(torch.isnan(dw[:, 32:64]).all()) and not bool(torch.isnan(dw[:, :32]).any()) and not bool(torch.isnan(dw[:, 64:]).any())
+    for fmt in ("int8", "e4m3"):
+        for a in (big[:64], big[:64, :5]):
+            dw = native.gemm_tn_ckpt(a, native.ckpt_pack(x, fmt))
+            assert bool(torch.isnan(dw[:, 32:64]).all()) and not bool(torch.isnan(dw[:, :32]).any()) and not bool(torch.isnan(dw[:, 64:]).any())
+    # one row whose codes have another unit stride
+    row = native.ActCheckpoint(kept.codes[:1].t().repeat(1, 2)[:, :1].t(), kept.scales[:1], 256)
+    assert torch.equal(native.ckpt_unpack(row).cpu(), v[:1])
 
 
 def pq_case(n, num_pq, k, d, fmt, seed, skew=1.0):

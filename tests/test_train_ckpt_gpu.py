@@ -118,6 +118,11 @@ def test_lookup_gradient_against_differences_and_formula(pkg, dev):
     half = books.detach().to(torch.bfloat16).requires_grad_(True)
     (grad16,) = torch.autograd.grad(pkg.code_lookup(idx, half, 1.5), half, g.to(torch.bfloat16))
     assert grad16.dtype == torch.bfloat16 and float((grad16.float() - grad).norm() / grad.norm()) < 2 * U_BF16
+    # through the gradient once more: d <lookup(B)^T g, v> / d g = lookup(v)
+    g2 = g.clone().requires_grad_(True)
+    (again,) = torch.autograd.grad(pkg.code_lookup(idx, books, 1.5), books, g2, create_graph=True)
+    (back,) = torch.autograd.grad(again, g2, v)
+    assert torch.equal(back, pkg.code_lookup(idx, v, 1.5))
     # the same code map twice, and one gradient for all rows (a broadcast)
     total = pkg.code_lookup(idx, books, 1.0).sum() + pkg.code_lookup(idx, books, 2.0).sum()
     (grad,) = torch.autograd.grad(total, books)
