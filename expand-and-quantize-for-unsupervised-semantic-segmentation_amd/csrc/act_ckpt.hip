@@ -1,6 +1,7 @@
 // 8-bit activation checkpoints: equss_ckpt_pack writes an activation as codes and scale bytes (ckpt.h), equss_ckpt_unpack reads
-// it back.  Both are one pass over memory and bound by it: a lane owns 8 consecutive channels, so four lanes share a block of
-// 32, its largest magnitude is two lane exchanges, and a wave stores 512 codes as one run.
+// it back.  Both are one pass over memory and bound by it: a lane owns 16 bytes of the activation (4 channels in fp32, 8 in 16
+// bits), so that a wave reads and writes whole kilobytes; 8 or 4 lanes share a block of 32, whose largest magnitude is 3 or 2
+// lane exchanges.
 //
 // Per block: k is the smallest integer >= -110 for which the largest magnitude, times 2^-k and rounded, does not pass 127
 // (int8) or 448 (e4m3).  With e = floor(log2(amax)), amax 2^-(e-6) lies in [64, 128) and amax 2^-(e-8) in [256, 512): the
@@ -14,7 +15,6 @@ typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x4u2 __attribute__((ext_vector_type(4), aligned(2)));
 
 constexpr int kThreads = 256;
-constexpr int kVec = 8;          // channels a lane
 
 template <int T> struct Elem;    // 0 fp32, 1 bf16, 2 fp16
 template <> struct Elem<0> { typedef float type; };
@@ -28,13 +28,15 @@ __device__ __forceinline__ float to_f32(typename Elem<T>::type v) {
     else return (float)v;
 }
 
-// 8 consecutive elements of a row; the rows of an odd width start at any element, which global loads take as they are
+template <int T> constexpr int kVec = T == 0 ? 4 : 8;      // channels a lane
+
+// a lane's channels of a row; the rows of an odd width start at any element, which global loads take as they are
 template <int T>
-__device__ __forceinline__ void load8(const typename Elem<T>::type* p, float (&x)[kVec]) {
+__device__ __forceinline__ void load_vec(const typename Elem<T>::type* p, float (&x)[kVec<T>]) {
     if constexpr (T == 0) {
-        const f32x4u a = *reinterpret_cast<const f32x4u*>(p), b = *reinterpret_cast<const f32x4u*>(p + 4);
+        const f32x4u a = *reinterpret_cast<const f32x4u*>(p);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { x[i] = a[i]; x[4 + i] = b[i]; }
+        for (int i = 0; i < 4; ++i) x[i] = a[i];
     } else {
         const u32x4u2 w = *reinterpret_cast<const u32x4u2*>(p);
 #pragma unroll
@@ -53,13 +55,12 @@ __device__ __forceinline__ void load8(const typename Elem<T>::type* p, float (&x
 }
 
 template <int T>
-__device__ __forceinline__ void store8(typename Elem<T>::type* p, const float (&x)[kVec]) {
+__device__ __forceinline__ void store_vec(typename Elem<T>::type* p, const float (&x)[kVec<T>]) {
     if constexpr (T == 0) {
-        f32x4u a, b;
+        f32x4u a;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { a[i] = x[i]; b[i] = x[4 + i]; }
+        for (int i = 0; i < 4; ++i) a[i] = x[i];
         *reinterpret_cast<f32x4u*>(p) = a;
-        *reinterpret_cast<f32x4u*>(p + 4) = b;
     } else {
         u32x4u2 w;
 #pragma unroll
@@ -74,7 +75,7 @@ __device__ __forceinline__ void store8(typename Elem<T>::type* p, const float (&
     }
 }
 
-// A workgroup walks `per_wg` units of 8 channels, units_row of them a row (padded to whole blocks).  A unit's row within the
+// A workgroup walks rows_wg rows in units of a lane's channels, units_row of them a row (padded to whole blocks).  A unit's row within the
 // workgroup's rows is unit / units_row by one high multiplication: magic = ceil(2^32 / units_row) is exact while
 // unit * units_row < 2^32; rows of more units than that have a workgroup to themselves (magic = 0).
 struct Walk {
@@ -83,51 +84,53 @@ struct Walk {
     uint32_t magic;
 };
 
-__device__ __forceinline__ void place(const Walk& w, int64_t row0, uint32_t unit, int64_t& row, int& col) {
+__device__ __forceinline__ void place(const Walk& w, int vec, int64_t row0, uint32_t unit, int64_t& row, int& col) {
     const uint32_t r = __umulhi(unit, w.magic);
     row = row0 + r;
-    col = (int)(unit - r * (uint32_t)w.units_row) * kVec;
+    col = (int)(unit - r * (uint32_t)w.units_row) * vec;
 }
 
 template <int T, bool E4M3, bool KEEP>
 __global__ __launch_bounds__(kThreads) void ckpt_pack_kernel(const typename Elem<T>::type* __restrict__ x, int64_t ld_x,
                                                             uint8_t* __restrict__ codes, int64_t ld_codes,
                                                             uint8_t* __restrict__ scales, int64_t ld_scales, const Walk w) {
+    constexpr int V = kVec<T>, LANES = equss::kCkptBlock / V;
     const int64_t row0 = (int64_t)blockIdx.x * w.rows_wg;
     const int64_t left = w.rows - row0;
     const uint32_t units = (uint32_t)((left < w.rows_wg ? left : w.rows_wg) * w.units_row);
-    // units_row is a multiple of 4 and so is a workgroup's first unit: the four lanes of a block are neighbours, all in or all out
+    // units_row is a multiple of a block's LANES and a workgroup starts with a row: these lanes are neighbours, all in or all out
     for (uint32_t u = threadIdx.x; u < units; u += kThreads) {
         int64_t row;
         int col;
-        place(w, row0, u, row, col);
+        place(w, V, row0, u, row, col);
         const typename Elem<T>::type* src = x + row * ld_x + col;
-        float v[kVec];
-        if (col + kVec <= w.width) load8<T>(src, v);
+        float v[V];
+        if (col + V <= w.width) load_vec<T>(src, v);
         else {
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) v[i] = col + i < w.width ? to_f32<T>(src[i]) : 0.f;
+            for (int i = 0; i < V; ++i) v[i] = col + i < w.width ? to_f32<T>(src[i]) : 0.f;
         }
         // the largest magnitude as an integer: the bits of non-negative floats order like their values, infinity and NaN on top
         uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) {
+        for (int i = 0; i < V; ++i) {
             const uint32_t a = __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu;
             m = a > m ? a : m;
         }
-        uint32_t o = (uint32_t)__shfl_xor((int)m, 1, 64);
-        m = o > m ? o : m;
-        o = (uint32_t)__shfl_xor((int)m, 2, 64);
-        m = o > m ? o : m;
+#pragma unroll
+        for (int o = 1; o < LANES; o *= 2) {
+            const uint32_t other = (uint32_t)__shfl_xor((int)m, o, 64);
+            m = other > m ? other : m;
+        }
         const bool lost = m >= 0x7f800000u;
         int k = (int)(m >> 23) - 127 - (E4M3 ? 8 : 6);
         k = k < equss::kCkptMinExp ? equss::kCkptMinExp : k;
         const float peak = __builtin_bit_cast(float, m) * equss::ckpt_scale((uint32_t)(127 - k));
         if (E4M3 ? peak > 464.f : peak >= 127.5f) ++k;
         const float inv = equss::ckpt_scale((uint32_t)(127 - k));
-        uint32_t out[2];
+        uint32_t out[V / 4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < V / 4; ++h) {
             float s[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[i] = v[4 * h + i] * inv;
@@ -156,9 +159,10 @@ __global__ __launch_bounds__(kThreads) void ckpt_pack_kernel(const typename Elem
                 }
             }
         }
-        if (lost) out[0] = out[1] = 0;
-        *reinterpret_cast<uint2*>(codes + row * ld_codes + col) = make_uint2(out[0], out[1]);
-        if ((u & 3) == 0) scales[row * ld_scales + col / equss::kCkptBlock] = (uint8_t)(lost ? equss::kCkptNanByte : k + 127);
+        uint8_t* dst = codes + row * ld_codes + col;
+        if constexpr (V == 4) *reinterpret_cast<uint32_t*>(dst) = lost ? 0u : out[0];
+        else *reinterpret_cast<uint2*>(dst) = lost ? make_uint2(0, 0) : make_uint2(out[0], out[V / 4 - 1]);
+        if ((u & (LANES - 1)) == 0) scales[row * ld_scales + col / equss::kCkptBlock] = (uint8_t)(lost ? equss::kCkptNanByte : k + 127);
     }
 }
 
@@ -166,25 +170,36 @@ template <int T, bool E4M3>
 __global__ __launch_bounds__(kThreads) void ckpt_unpack_kernel(const uint8_t* __restrict__ codes, int64_t ld_codes,
                                                               const uint8_t* __restrict__ scales, int64_t ld_scales,
                                                               typename Elem<T>::type* __restrict__ out, int64_t ld_out, const Walk w) {
+    constexpr int V = kVec<T>;
     const int64_t row0 = (int64_t)blockIdx.x * w.rows_wg;
     const int64_t left = w.rows - row0;
     const uint32_t units = (uint32_t)((left < w.rows_wg ? left : w.rows_wg) * w.units_row);
     for (uint32_t u = threadIdx.x; u < units; u += kThreads) {
         int64_t row;
         int col;
-        place(w, row0, u, row, col);
+        place(w, V, row0, u, row, col);
         if (col >= w.width) continue;
-        const uint2 q = *reinterpret_cast<const uint2*>(codes + row * ld_codes + col);
+        const uint32_t* q = reinterpret_cast<const uint32_t*>(codes + row * ld_codes + col);
+        uint32_t c[V / 4];
+        if constexpr (V == 4) c[0] = *q;
+        else {
+            const uint2 w2 = *reinterpret_cast<const uint2*>(q);
+            c[0] = w2.x;
+            c[V / 4 - 1] = w2.y;
+        }
         const float s = equss::ckpt_scale(scales[row * ld_scales + col / equss::kCkptBlock]);
-        const f32x4 a = equss::ckpt_decode4<E4M3>(q.x), b = equss::ckpt_decode4<E4M3>(q.y);
-        float v[kVec];
+        float v[V];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { v[i] = a[i] * s; v[4 + i] = b[i] * s; }
+        for (int h = 0; h < V / 4; ++h) {
+            const f32x4 d = equss::ckpt_decode4<E4M3>(c[h]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[4 * h + i] = d[i] * s;
+        }
         typename Elem<T>::type* dst = out + row * ld_out + col;
-        if (col + kVec <= w.width) store8<T>(dst, v);
+        if (col + V <= w.width) store_vec<T>(dst, v);
         else {
 #pragma unroll
-            for (int i = 0; i < kVec; ++i)
+            for (int i = 0; i < V; ++i)
                 if (col + i < w.width) {
                     if constexpr (T == 0) dst[i] = v[i];
                     else if constexpr (T == 1) dst[i] = equss::f2bf(v[i]);
@@ -210,12 +225,16 @@ int checks(const char* what, const void* x, int type, int64_t ld, const void* co
     return EQUSS_OK;
 }
 
-// About 8 units a lane and workgroup: enough loads in flight at eight workgroups a CU, and > 256 workgroups from 2 MB of codes on.
-bool walk(Walk& w, int64_t rows, int width, int64_t& grid) {
+// Four units a lane (102400 x 768 bf16, int8: 44 us; 45 with two, 46 with eight, 53 with sixteen), and > 256 workgroups from a
+// megabyte on.  Measured at 102400 rows: 768 bf16 written in 43 us (5.5 TB/s of its 238 MB) and read back in 38 us (6.3 TB/s),
+// 1024 fp32 in 96 and 92 us (5.5 and 5.8 TB/s of 531 MB; 104 and 142 us with eight channels a lane there too, whose two loads
+// and stores leave every other 16 bytes to the next instruction); a copy of 1 GiB runs at 5.15 TB/s.
+bool walk(Walk& w, int64_t rows, int width, int type, int64_t& grid) {
+    const int vec = type == EQUSS_F32 ? 4 : 8;
     w.rows = rows;
     w.width = width;
-    w.units_row = (width + equss::kCkptBlock - 1) / equss::kCkptBlock * (equss::kCkptBlock / kVec);
-    int64_t r = 8 * kThreads / w.units_row;
+    w.units_row = (width + equss::kCkptBlock - 1) / equss::kCkptBlock * (equss::kCkptBlock / vec);
+    int64_t r = 4 * kThreads / w.units_row;
     const int64_t spread = (rows + 1023) / 1024;   // few rows: as many workgroups as rows
     if (r > spread) r = spread;
     if (r < 1) r = 1;
@@ -234,7 +253,7 @@ extern "C" int equss_ckpt_pack(const void* x, int type, int64_t ld_x, void* code
     if (rc != EQUSS_OK || rows == 0) return rc;
     Walk w;
     int64_t grid;
-    if (!walk(w, rows, width, grid)) return equss::fail(EQUSS_E_UNSUPPORTED, "equss_ckpt_pack: %lld rows of %d channels", (long long)rows, width);
+    if (!walk(w, rows, width, type, grid)) return equss::fail(EQUSS_E_UNSUPPORTED, "equss_ckpt_pack: %lld rows of %d channels", (long long)rows, width);
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
 #define EQUSS_PACK(T, E, K)                                                                                                       \
     hipLaunchKernelGGL((ckpt_pack_kernel<T, E, K>), dim3((unsigned)grid), dim3(kThreads), 0, s,                                   \
@@ -257,7 +276,7 @@ extern "C" int equss_ckpt_unpack(const void* codes, int64_t ld_codes, const void
     if (rc != EQUSS_OK || rows == 0) return rc;
     Walk w;
     int64_t grid;
-    if (!walk(w, rows, width, grid)) return equss::fail(EQUSS_E_UNSUPPORTED, "equss_ckpt_unpack: %lld rows of %d channels", (long long)rows, width);
+    if (!walk(w, rows, width, type, grid)) return equss::fail(EQUSS_E_UNSUPPORTED, "equss_ckpt_unpack: %lld rows of %d channels", (long long)rows, width);
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
 #define EQUSS_UNPACK(T, E)                                                                                                        \
     hipLaunchKernelGGL((ckpt_unpack_kernel<T, E>), dim3((unsigned)grid), dim3(kThreads), 0, s, reinterpret_cast<const uint8_t*>(codes), \

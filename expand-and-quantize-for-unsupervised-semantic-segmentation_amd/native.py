@@ -205,11 +205,11 @@ def _stream(t):
     """The current HIP stream of ``t``'s device.  Kernels launch on the CURRENT device, so that device
     must be the tensor's: a launch with a foreign device's pointers and stream handle would corrupt
     memory silently, hence the loud failure (one process per GPU, as torchrun sets it up, never trips it)."""
-    index = t.device.index
-    if index is not None and index != torch.cuda.current_device():
+    index = t.get_device()          # (-1 for a host tensor, which the callers refuse)
+    if index != torch.cuda.current_device():
         raise EqussError(f"tensor lives on {t.device} but the current device is cuda:{torch.cuda.current_device()}; "
                          f"wrap the call in `with torch.cuda.device({t.device.index}):`")
-    if _raw_stream is not None and index is not None:
+    if _raw_stream is not None:
         return ctypes.c_void_p(_raw_stream(index))
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
@@ -694,7 +694,7 @@ class ActCheckpoint:
 
     @property
     def rows(self):
-        return self.codes.shape[0]
+        return self.codes.size(0)
 
     @property
     def fmt(self):
@@ -776,9 +776,10 @@ def ckpt_unpack(ckpt, dtype=torch.float32):
     if dtype not in _ELEM_TYPES:
         raise ValueError("ckpt_unpack: dtype must be float32, bfloat16 or float16")
     codes, ld_codes, scales, ld_scales = _ckpt_parts(ckpt)
-    out = codes.new_empty((ckpt.rows, ckpt.width), dtype=dtype)
-    _check(load_library().equss_ckpt_unpack(_at(codes), ld_codes, _at(scales), ld_scales, _at(out), _ELEM_TYPES[dtype], ckpt.width,
-                                            ckpt.rows, ckpt.width, CKPT_FORMATS[ckpt.fmt], _stream(codes)), "equss_ckpt_unpack")
+    rows, width = codes.size(0), ckpt.width
+    out = codes.new_empty((rows, width), dtype=dtype)
+    _check(load_library().equss_ckpt_unpack(codes.data_ptr(), ld_codes, scales.data_ptr(), ld_scales, out.data_ptr(), _ELEM_TYPES[dtype],
+                                            width, rows, width, CKPT_FORMATS[ckpt.fmt], _stream(codes)), "equss_ckpt_unpack")
     return out
 
 

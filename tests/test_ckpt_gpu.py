@@ -181,6 +181,11 @@ def test_weight_gradient_takes_views_and_no_rows(native, dev):
         for lo, hi in ((0, 256), (64, 128), (224, 256)):
             got = native.gemm_tn_ckpt(a, kept.columns(lo, hi))
             assert torch.equal(got.cpu(), (a.cpu().to(F64).t() @ v[:, lo:hi].to(F64)).to(F32))
+    far = torch.zeros(600, 2_000_000, dtype=torch.bfloat16, device=dev)      # rows too far apart for 32-bit offsets
+    far[:500, 1_000_001:1_000_131] = big[:, :130]
+    got = native.gemm_tn_ckpt(far[:500, 1_000_001:1_000_131], kept, want_bias=True)
+    assert torch.equal(got[0].cpu(), (big[:, :130].cpu().to(F64).t() @ v.to(F64)).to(F32)) and torch.equal(got[1].cpu(), big[:, :130].cpu().to(F64).sum(0).to(F32))
+    del far
     dw, db = native.gemm_tn_ckpt(big[:0], native.ckpt_pack(torch.zeros(0, 48, device=dev)), want_bias=True)
     assert dw.shape == (300, 48) and not bool(dw.any()) and not bool(db.any())
     # a block of NaN spoils its own columns only
@@ -312,3 +317,41 @@ def test_checkpoint_calls_on_a_side_stream_and_in_a_replayed_graph(native, dev):
         assert all(torch.equal(x, y) for x, y in zip(held, eager)), i
         native.pq_st_backward_ckpt(native.ckpt_pack(z[:2500]), books, idx[:, :2500], None, g_vq, 0.25, 1.0)
         torch.cuda.synchronize()
+
+
+def test_offsets_past_32_bits(native, dev):
+    """Row buffers of more than 2^31 elements: what the calls do with the last rows of them is what they do with these rows alone."""
+    rows, num_pq, d, k, tail = 2_200_000, 8, 128, 64, 1500
+    width = num_pq * d
+    assert rows * width > 2 ** 31
+    x = torch.randn(tail, width, device=dev).to(torch.bfloat16)
+    big = torch.zeros(rows, width, dtype=torch.bfloat16, device=dev)
+    big[-tail:] = x
+    for fmt in ("int8", "e4m3"):
+        kept, small = native.ckpt_pack(big, fmt), native.ckpt_pack(x, fmt)
+        last = native.ActCheckpoint(kept.codes[-tail:], kept.scales[-tail:], width)
+        assert torch.equal(last.codes.view(torch.uint8), small.codes.view(torch.uint8)) and torch.equal(last.scales, small.scales)
+        back = native.ckpt_unpack(kept, torch.bfloat16)
+        assert torch.equal(back[-tail:], native.ckpt_unpack(small, torch.bfloat16)) and not bool(back[:-tail].any())
+        del back
+    # weight gradient: whole numbers in the last rows only (NaN-free zeros before), exact whatever the row ranges
+    a = torch.zeros(rows, 64, dtype=torch.bfloat16, device=dev)
+    a[-tail:] = torch.randint(-2, 3, (tail, 64), device=dev).to(torch.bfloat16)
+    big[-tail:] = torch.randint(-15, 16, (tail, width), device=dev).to(torch.bfloat16)
+    kept = native.ckpt_pack(big, "int8")
+    dw, db = native.gemm_tn_ckpt(a, kept, want_bias=True)
+    assert torch.equal(dw.to(F64), a[-tail:].to(F64).t() @ big[-tail:].to(F64)) and torch.equal(db.to(F64), a[-tail:].to(F64).sum(0))
+    # lookup and its gradient
+    idx = torch.randint(-1, k, (num_pq, rows), device=dev)
+    books = torch.randn(num_pq, k, d, device=dev).to(torch.bfloat16)
+    assert torch.equal(native.code_lookup(idx, books)[-tail:], native.code_lookup(idx[:, -tail:], books))
+    assert torch.equal(native.code_lookup_grad(big, idx, k), native.code_lookup_grad(big[-tail:], idx[:, -tail:], k))
+    # quantiser: a row's gradient is its own (no vq loss here); the codebooks' is zero without it
+    idx.clamp_(min=0)
+    books, zero = books.float(), torch.zeros((), device=dev)
+    g = torch.zeros(rows, width, device=dev)
+    g[-tail:] = torch.randn(tail, width, device=dev)
+    gz, gb = native.pq_st_backward_ckpt(kept, books, idx, g, zero, 0.25, 1.0)
+    last = native.ActCheckpoint(kept.codes[-tail:].contiguous(), kept.scales[-tail:].contiguous(), width)
+    want, _ = native.pq_st_backward_ckpt(last, books, idx[:, -tail:], g[-tail:], zero, 0.25, 1.0)
+    assert torch.equal(gz[-tail:], want) and not bool(gz[:-tail].any()) and not bool(gb.any())
