@@ -28,39 +28,43 @@ __device__ __forceinline__ void pairs_at(const Source& s, int p, int64_t i, int 
     }
 }
 
-__global__ __launch_bounds__(256) void code_count_kernel(const Source s, uint32_t* __restrict__ table, int chunk_rows, int shift, int bits) {
+constexpr int kCountThreads = 1024;
+
+__global__ __launch_bounds__(kCountThreads) void code_count_kernel(const Source s, uint32_t* __restrict__ table, int chunk_rows, int shift, int bits) {
     __shared__ uint32_t hist[equss::kMaxBins];
+    constexpr int B = 8;
     const int bins = 1 << bits, p = blockIdx.y, chunk = blockIdx.x, chunks = gridDim.x;
-    for (int b = threadIdx.x; b < bins; b += 256) hist[b] = 0;
+    for (int b = threadIdx.x; b < bins; b += kCountThreads) hist[b] = 0;
     __syncthreads();
     const int64_t i0 = (int64_t)chunk * chunk_rows, i1 = i0 + chunk_rows < s.rows ? i0 + chunk_rows : s.rows;
-    for (int64_t i = i0 + threadIdx.x; i < i1; i += 256 * 8) {
-        CodePair pr[8];
-        pairs_at<8>(s, p, i, 256, i1, pr);
+    for (int64_t i = i0 + threadIdx.x; i < i1; i += kCountThreads * B) {
+        CodePair pr[B];
+        pairs_at<B>(s, p, i, kCountThreads, i1, pr);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (i + j * 256 < i1) atomicAdd(&hist[(pr[j].code >> shift) & (bins - 1)], 1u);
+        for (int j = 0; j < B; ++j)
+            if (i + j * kCountThreads < i1) atomicAdd(&hist[(pr[j].code >> shift) & (bins - 1)], 1u);
     }
     __syncthreads();
     uint32_t* row = table + ((int64_t)p * chunks + chunk) * bins;
-    for (int b = threadIdx.x; b < bins; b += 256) row[b] = hist[b];
+    for (int b = threadIdx.x; b < bins; b += kCountThreads) row[b] = hist[b];
 }
 
-// A wave owns a quarter of the chunk, so that ranks follow the row order.  starts: (num_pq, K + 1), written by the last pass of
-// one-pass sorts (whose bins are the codes), or null.  What this kernel waits for is latency, so loads come in batches: the
-// wave's pairs eight times 64 at once (kept for the second look at them where that is all of them) and the chunks' counts
-// up to 64 at once.
-template <int PER>                                      // bins a thread: bins <= 256 PER
-__global__ __launch_bounds__(256) void code_place_kernel(const Source s, const uint32_t* __restrict__ table, CodePair* __restrict__ dst,
-                                                        uint32_t* __restrict__ starts, int chunk_rows, int shift, int bits) {
-    constexpr int B = 8, NB = PER <= 2 ? 64 / PER : 16;
-    __shared__ uint32_t base[4][256 * PER];             // next place of every bin, for each wave
-    __shared__ uint32_t first[256 * PER];               // all of the bin's pairs, then where they start
-    __shared__ uint32_t wave_sum[4];
+// Every wave owns a share of the chunk, so that ranks follow the row order.  starts: (num_pq, K + 1), written by the last pass of
+// one-pass sorts (whose bins are the codes), or null.  What this kernel waits for is latency: a wave's pairs are loaded eight
+// times 64 at once (and kept where that is all of them), the chunks' counts sixteen at once.  Many waves a workgroup make few
+// chunks, i.e. few counts to read for each: 102400 rows, 8 sub-spaces, both kernels: 15.8 us with 16 waves and 15 chunks, 18.3 us
+// with 4 waves and 50 chunks; two kernels that only launch and load take 9.
+template <int WAVES, int BINS>                          // bins <= BINS, a multiple or a fraction of the threads
+__global__ __launch_bounds__(64 * WAVES) void code_place_kernel(const Source s, const uint32_t* __restrict__ table, CodePair* __restrict__ dst,
+                                                               uint32_t* __restrict__ starts, int chunk_rows, int shift, int bits) {
+    constexpr int B = 8, THREADS = 64 * WAVES, PER = BINS > THREADS ? BINS / THREADS : 1, NB = 16;
+    __shared__ uint32_t base[WAVES][BINS];              // next place of every bin, for each wave
+    __shared__ uint32_t first[PER * THREADS];           // all of the bin's pairs, then where they start
+    __shared__ uint32_t wave_sum[WAVES];
     const int bins = 1 << bits, p = blockIdx.y, chunk = blockIdx.x, chunks = gridDim.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t i0 = (int64_t)chunk * chunk_rows + (int64_t)wave * (chunk_rows / 4);
-    int64_t i1 = i0 + chunk_rows / 4;
+    const int64_t i0 = (int64_t)chunk * chunk_rows + (int64_t)wave * (chunk_rows / WAVES);
+    int64_t i1 = i0 + chunk_rows / WAVES;
     if (i1 > s.rows) i1 = s.rows;
     CodePair held[B];
     auto fetch = [&](int64_t i) __attribute__((always_inline)) { pairs_at<B>(s, p, i + lane, 64, i1, held); };
@@ -69,28 +73,29 @@ __global__ __launch_bounds__(256) void code_place_kernel(const Source s, const u
     uint32_t before[PER], total[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) before[j] = total[j] = 0;
-    // (bins is at least 2 and a power of two: a thread without a bin reads one of the others')
-    const int at0 = tid & (bins - 1);
-    for (int c0 = 0; c0 < chunks; c0 += NB) {
-        uint32_t n[PER][NB];
+    if (tid < bins) {                                   // (with more than one bin a thread there are exactly PER)
+        for (int c0 = 0; c0 < chunks; c0 += NB) {
+            uint32_t n[PER][NB];
 #pragma unroll
-        for (int j = 0; j < PER; ++j)
+            for (int j = 0; j < PER; ++j)
 #pragma unroll
-            for (int i = 0; i < NB; ++i) n[j][i] = rows_p[(c0 + i < chunks ? c0 + i : chunks - 1) * bins + at0 + 256 * j];
+                for (int i = 0; i < NB; ++i) n[j][i] = rows_p[(c0 + i < chunks ? c0 + i : chunks - 1) * bins + tid + THREADS * j];
 #pragma unroll
-        for (int j = 0; j < PER; ++j)
+            for (int j = 0; j < PER; ++j)
 #pragma unroll
-            for (int i = 0; i < NB; ++i) {
-                before[j] += c0 + i < chunk ? n[j][i] : 0u;
-                total[j] += c0 + i < chunks ? n[j][i] : 0u;
-            }
+                for (int i = 0; i < NB; ++i) {
+                    before[j] += c0 + i < chunk ? n[j][i] : 0u;
+                    total[j] += c0 + i < chunks ? n[j][i] : 0u;
+                }
+        }
     }
-    if (tid >= bins) total[0] = 0;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        first[tid + 256 * j] = total[j];
+        first[tid + THREADS * j] = total[j];
+        if (tid < BINS) {
 #pragma unroll
-        for (int v = 0; v < 4; ++v) base[v][tid + 256 * j] = 0;
+            for (int v = 0; v < WAVES; ++v) base[v][tid + THREADS * j] = 0;
+        }
     }
     __syncthreads();
     for (int64_t i = i0; i < i1; i += 64 * B) {
@@ -126,12 +131,15 @@ __global__ __launch_bounds__(256) void code_place_kernel(const Source s, const u
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        uint32_t at = first[tid + 256 * j] + before[j];
+        if (tid < BINS) {
+            uint32_t at = first[tid + THREADS * j] + before[j], n[WAVES];
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            const uint32_t n = base[v][tid + 256 * j];
-            base[v][tid + 256 * j] = at;
-            at += n;
+            for (int v = 0; v < WAVES; ++v) n[v] = base[v][tid + THREADS * j];
+#pragma unroll
+            for (int v = 0; v < WAVES; ++v) {
+                base[v][tid + THREADS * j] = at;
+                at += n[v];
+            }
         }
     }
     __syncthreads();
@@ -143,8 +151,9 @@ __global__ __launch_bounds__(256) void code_place_kernel(const Source s, const u
 #pragma unroll
         for (int j = 0; j < B; ++j) {
             const bool in = i + j * 64 + lane < i1;
-            const uint32_t digit = (held[j].code >> shift) & (bins - 1);
             uint64_t same = __ballot(in);
+            if (same == 0) break;
+            const uint32_t digit = (held[j].code >> shift) & (bins - 1);
             for (int b = 0; b < bits; ++b) {
                 const uint64_t set = __ballot((digit >> b) & 1);
                 same &= (digit >> b) & 1 ? set : ~set;
@@ -194,9 +203,12 @@ bool sort_plan(SortPlan& s, int64_t rows, int num_pq, int64_t K, int d) {
         s.bits[i] = (left + s.passes - i - 1) / (s.passes - i);
         left -= s.bits[i];
     }
-    int64_t chunk = (rows + 63) / 64;                      // at most 64 chunks: every one reads the others' counts
-    if (chunk < 2048) chunk = 2048;
-    s.chunk_rows = (int)((chunk + 255) / 256 * 256);
+    // chunks of up to 8192 rows, 512 for each of 16 waves, and shorter ones as long as there are no more than 16; at most 64 of
+    // them in all: every one reads the others' counts
+    int64_t chunk = (rows + 15) / 16;
+    if (chunk > 8192) chunk = 8192;
+    if (chunk < (rows + 63) / 64) chunk = (rows + 63) / 64;
+    s.chunk_rows = (int)((chunk + 1023) / 1024 * 1024);
     s.chunks = (int)((rows + s.chunk_rows - 1) / s.chunk_rows);
     // tiles of 64, or as short as 8 where that leaves the chip half empty: 4096 waves
     const int64_t lanes = d >= 256 ? 64 : (d + 3) / 4;
@@ -224,15 +236,14 @@ int sort_launch(const SortPlan& s, const IndexView& index, char* ws, size_t* pai
     int shift = 0;
     for (int i = 0; i < s.passes; ++i) {
         dst = (i & 1) ? s.pairs_b : s.pairs_a;
-        hipLaunchKernelGGL(code_count_kernel, grid, dim3(256), 0, stream, src, table, s.chunk_rows, shift, s.bits[i]);
+        hipLaunchKernelGGL(code_count_kernel, grid, dim3(kCountThreads), 0, stream, src, table, s.chunk_rows, shift, s.bits[i]);
         int rc = check_launch("code_count_kernel");
         if (rc != EQUSS_OK) return rc;
         CodePair* to = reinterpret_cast<CodePair*>(ws + dst);
         uint32_t* runs = s.passes == 1 ? starts : nullptr;
-        if (s.bits[i] <= 8) hipLaunchKernelGGL(code_place_kernel<1>, grid, dim3(256), 0, stream, src, table, to, runs, s.chunk_rows, shift, s.bits[i]);
-        else if (s.bits[i] == 9) hipLaunchKernelGGL(code_place_kernel<2>, grid, dim3(256), 0, stream, src, table, to, runs, s.chunk_rows, shift, s.bits[i]);
-        else if (s.bits[i] == 10) hipLaunchKernelGGL(code_place_kernel<4>, grid, dim3(256), 0, stream, src, table, to, runs, s.chunk_rows, shift, s.bits[i]);
-        else hipLaunchKernelGGL(code_place_kernel<8>, grid, dim3(256), 0, stream, src, table, to, runs, s.chunk_rows, shift, s.bits[i]);
+        if (s.bits[i] <= 9) hipLaunchKernelGGL((code_place_kernel<16, 512>), grid, dim3(1024), 0, stream, src, table, to, runs, s.chunk_rows, shift, s.bits[i]);
+        else if (s.bits[i] == 10) hipLaunchKernelGGL((code_place_kernel<8, 1024>), grid, dim3(512), 0, stream, src, table, to, runs, s.chunk_rows, shift, s.bits[i]);
+        else hipLaunchKernelGGL((code_place_kernel<4, 2048>), grid, dim3(256), 0, stream, src, table, to, runs, s.chunk_rows, shift, s.bits[i]);
         rc = check_launch("code_place_kernel");
         if (rc != EQUSS_OK) return rc;
         shift += s.bits[i];
