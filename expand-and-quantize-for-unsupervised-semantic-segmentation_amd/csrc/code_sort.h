@@ -170,58 +170,62 @@ __global__ __launch_bounds__(256) void code_accumulate_kernel(const Op op, const
     }
 }
 
-// A wave owns a code; the chain of partial sums of a long run is shared by the workgroup's four waves.
-template <int LPR>
-__global__ __launch_bounds__(256) void code_join_kernel(const WalkArgs w) {
-    constexpr int SLOTS = 64 / LPR, kLong = 16 * SLOTS;
-    __shared__ f32x4 share[4 * 64];
+// WAVES = 4: a wave owns a code, and the chain of partial sums of a long run is shared by the workgroup's four waves.  WAVES = 16,
+// where there are few codes, i.e. long runs: a workgroup owns a code (102045 rows, 5 x 2 x 32, gradient of a lookup: 42 us, 65 us
+// with four waves; 102400 rows, 8 x 256 x 128: 100 / 96 us, hence at most 1024 codes).
+template <int LPR, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void code_join_kernel(const WalkArgs w) {
+    constexpr int SLOTS = 64 / LPR, CODES = WAVES == 4 ? 4 : 1, kLong = 16 * SLOTS, F = 8;
+    __shared__ f32x4 share[WAVES][LPR];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, slot = lane / LPR;
     const int p = blockIdx.y, col = (int)blockIdx.z * 256 + (lane % LPR) * 4;
     const bool live = col < w.d, whole = (w.d & 3) == 0;
     const uint32_t* starts = w.starts + (int64_t)p * ((int64_t)w.K + 1);
     const float* part = w.partial + (int64_t)p * w.tiles * 2 * w.dpad + (live ? col : 0);
     float* out = w.out + (int64_t)p * w.K * w.d + col;
-    // link 0 is the first tile's tail, the others the following tiles' heads; sums of links first, first + step, ...
+    // link 0 is the first tile's tail, the others the following tiles' heads; the sum of links first, first + step, ... of all the
+    // groups of a wave, in every one of them
     auto chain = [&](int64_t ts, int64_t links, int64_t first, int64_t step) {
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-        for (int64_t j = first; j < links; j += 4 * step) {
-            f32x4 v[4];
+        for (int64_t j = first; j < links; j += F * step) {
+            f32x4 v[F];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < F; ++i) {
                 const int64_t l = j + i * step < links ? j + i * step : first;
                 v[i] = *reinterpret_cast<const f32x4*>(part + ((ts + l) * 2 + (l == 0 ? 1 : 0)) * w.dpad);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < F; ++i)
                 if (j + i * step < links) acc += v[i];
         }
+#pragma unroll
+        for (int o = 32; o >= LPR; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], o, 64);
         return acc;
     };
-    const int64_t k0 = (int64_t)blockIdx.x * 4;
-    int64_t at[5];
+    const int64_t k0 = (int64_t)blockIdx.x * CODES;
+    int64_t at[CODES + 1];
 #pragma unroll
-    for (int c = 0; c < 5; ++c) at[c] = starts[k0 + c <= (int64_t)w.K ? k0 + c : (int64_t)w.K];
+    for (int c = 0; c <= CODES; ++c) at[c] = starts[k0 + c <= (int64_t)w.K ? k0 + c : (int64_t)w.K];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
+    for (int c = 0; c < CODES; ++c) {
         const int64_t k = k0 + c;
         if (k >= (int64_t)w.K) break;                      // (uniform over the workgroup)
         const int64_t s = at[c], e = at[c + 1];
         const int64_t ts = s / w.tile, links = e > s ? (e - 1) / w.tile - ts + 1 : 0;
-        const bool far = links > kLong;
-        if (!far) {
+        if (links <= kLong) {
             if (wave != c || links == 1) continue;         // one tile held the whole run: it is written already
-            f32x4 acc = chain(ts, links, slot, SLOTS);
-#pragma unroll
-            for (int o = 32; o >= LPR; o >>= 1)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], o, 64);
+            const f32x4 acc = chain(ts, links, slot, SLOTS);
             if (slot == 0 && live) store_cols(out + k * w.d, acc, col, w.d, whole);
         } else {
-            share[wave * 64 + lane] = chain(ts, links, wave * SLOTS + slot, 4 * SLOTS);
+            const f32x4 mine = chain(ts, links, wave * SLOTS + slot, WAVES * SLOTS);
+            if (slot == 0) share[wave][lane] = mine;
             __syncthreads();
             if (wave == 0 && slot == 0 && live) {
                 f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-                for (int j = 0; j < 4 * SLOTS; ++j) acc += share[j * LPR + lane];
+#pragma unroll
+                for (int j = 0; j < WAVES; ++j) acc += share[j][lane];
                 store_cols(out + k * w.d, acc, col, w.d, whole);
             }
             __syncthreads();
@@ -407,7 +411,8 @@ int walk_launch_lpr(const Op& op, const SortPlan& s, const IndexView& index, cha
     else hipLaunchKernelGGL((code_accumulate_kernel<Op, LPR, 2>), grid, dim3(256), 0, stream, op, w);
     rc = check_launch("code_accumulate_kernel");
     if (rc != EQUSS_OK || !out) return rc;
-    hipLaunchKernelGGL((code_join_kernel<LPR>), dim3((s.K + 3) / 4, s.num_pq, cchunks), dim3(256), 0, stream, w);
+    if ((int64_t)s.K * s.num_pq <= 1024) hipLaunchKernelGGL((code_join_kernel<LPR, 16>), dim3(s.K, s.num_pq, cchunks), dim3(1024), 0, stream, w);
+    else hipLaunchKernelGGL((code_join_kernel<LPR, 4>), dim3((s.K + 3) / 4, s.num_pq, cchunks), dim3(256), 0, stream, w);
     return check_launch("code_join_kernel");
 }
 
