@@ -9,6 +9,7 @@
 // is applied to a on the same way.  The rows are split over workgroups; their partial tiles go to the workspace and a second
 // kernel adds them in a fixed order, so equal calls give equal bits.
 #include "ckpt.h"
+#include <math.h>
 
 namespace {
 
@@ -34,6 +35,8 @@ struct Args {
     int M, N, tiles_m, tiles_n, splits, bias_tiles, npad, mpad;
 };
 
+// ---- the narrow form: any M (the tiled form reads 8 columns of a at once) and any leading dimensions (its offsets within a row
+// range are 32 bits); 4 waves of 2 x 2 MFMA tiles, one stage ahead in registers and one in LDS
 template <bool E4M3, bool MASK>
 __global__ __launch_bounds__(kTnThreads, 2) void gemm_tn_ckpt_kernel(const Args g) {
     __shared__ __attribute__((aligned(16))) char smem[2 * kStageB];
@@ -188,7 +191,8 @@ __global__ __launch_bounds__(kTnThreads, 2) void gemm_tn_ckpt_kernel(const Args 
 }
 
 // ---- square tiles of TILE = 256 (8 waves, two a SIMD, one workgroup a CU) or 128 (4 waves, two workgroups a CU) of C, in
-// 2 x TILE / 64 waves of TILE / 64 x 2 MFMA tiles of 32 x 32; 32 rows a stage, four stages in LDS.  While a stage's fragments are multiplied,
+// 2 x TILE / 64 waves of TILE / 64 x 2 MFMA tiles of 32 x 32; 32 rows a stage, four stages in LDS.  While a stage's fragments are
+// multiplied,
 //   the fragments of the next half stage are read (the next stage's first half too: its writes are a barrier back),
 //   the stage after the next goes from registers through the conversion into its slot of LDS, and
 //   each of those registers is requested again from two stages further on (there are two sets of them: one stage of 32 rows
@@ -199,6 +203,10 @@ __global__ __launch_bounds__(kTnThreads, 2) void gemm_tn_ckpt_kernel(const Args 
 // Conversions, address arithmetic and the bias are what the matrix pipe waits for (counted: of 75 M issue cycles of the first
 // version with one wave a SIMD, the MFMAs took 39 M and other vector instructions 23 M, one after the other); hence two waves
 // a SIMD, constant LDS addresses and buffer loads.
+// 102400 rows, 1024 x 768, bias and join included: int8 164 us, e4m3 (whose conversion is one instruction for two values) 154 us,
+// 0.98 and 1.05 PFLOP/s; an 8192^3 bf16 library product runs at 1.25.  The loop alone is at 1.36: writing every CU's 256 KB of
+// accumulators as partial products and joining them takes the other 25 us.  Consecutive row ranges and tiles on one XCD: 164 us,
+// 184 dealt round (102400 rows, 384 x 384: 54 / 70).
 // Columns past M: the last chunk of 8 columns is read at M - 8, so that every load is whole and inside; its columns then
 // overlap the chunk before, both give the same sums, and both are written.  Columns past N lie in the checkpoint's padding or
 // are read from its last block; their sums are dropped.
@@ -521,14 +529,14 @@ Plan plan(int64_t rows, int M, int N, int tile) {
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
     // Row ranges: more of them shorten everybody's loop (32 rows take 0.35 us, 0.75 us with the large tile and all CUs at work),
     // but two or more need the join (6 us for its launch and what it waits for), and each writes and reads back a partial product
-    // (0.08 us + 1.1 us for a million elements).  The cheapest number, at most one round of workgroups.
-    const int64_t most = (tile == 256 ? 256 : 512) / tiles, steps = (rows + bk - 1) / bk;
-    int64_t splits = 1;
-    double best = 1e300;
-    for (int64_t s = 1; s <= (most > 1 ? most : 1) && (s == 1 || 4 * s <= steps); ++s) {   // at least four steps a workgroup
-        const double cost = (double)((steps + s - 1) / s) * (tile == 256 ? 0.75 : 0.35) + (s > 1 ? 6.0 + (double)s * (0.08 + 1.1e-6 * M * N) : 0.0);
-        if (cost < best) { best = cost; splits = s; }
-    }
+    // (0.08 us + 1.1 us for a million elements).  The cheapest number, at least four steps each, at most one round of workgroups;
+    // one where that is cheaper (512 rows, 1024 x 768: 11.5 us, 17.0 with two ranges).
+    const int64_t steps = (rows + bk - 1) / bk, round = (tile == 256 ? 256 : 512) / tiles;
+    const double step = tile == 256 ? 0.75 : 0.35, range = 0.08 + 1.1e-6 * M * N;
+    int64_t splits = (int64_t)(sqrt((double)steps * step / range) + 0.5);
+    if (splits > round) splits = round;
+    if (splits > steps / 4) splits = steps / 4;
+    if (splits <= 1 || (double)(steps - steps / splits) * step < 6.0 + (double)splits * range) splits = 1;
     p.rows_split = ((rows + splits - 1) / splits + bk - 1) / bk * bk;
     if (p.rows_split < bk) p.rows_split = bk;
     p.splits = (int)((rows + p.rows_split - 1) / p.rows_split);
@@ -540,8 +548,8 @@ Plan plan(int64_t rows, int M, int N, int tile) {
 
 int tile_of(int64_t rows, int M, int N) {
     if (M < 8) return 0;
-    // Measured (us, int8; 128 against 256): 25088 x 1024 x 768 64.9 / 62.7, 12544 x 1024 x 768 42.1 / 43.6, 102400 x 384 x 384
-    // 57.4 / 67.7, 102400 x 1024 x 768 217 / 164, 1024 x 1024 x 768 18.3 / 24.8: the large tile, which reads half as much LDS
+    // Measured (us, int8; 128 against 256): 25088 x 1024 x 768 65 / 63, 12544 x 1024 x 768 42 / 44, 102400 x 384 x 384 57 / 68,
+    // 102400 x 1024 x 768 217 / 164, 1024 x 1024 x 768 18 / 25: the large tile, which reads half as much LDS
     // for a product, pays where every CU has a long way to go.
     return (double)rows * M * N >= 2e10 && M > 128 && N > 128 ? 256 : 128;
 }
