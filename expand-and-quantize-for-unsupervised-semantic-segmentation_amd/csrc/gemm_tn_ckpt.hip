@@ -191,8 +191,8 @@ __global__ __launch_bounds__(kTnThreads, 2) void gemm_tn_ckpt_kernel(const Args 
 }
 
 // ---- square tiles of TILE = 256 (8 waves, two a SIMD, one workgroup a CU) or 128 (4 waves, two workgroups a CU) of C, in
-// 2 x TILE / 64 waves of TILE / 64 x 2 MFMA tiles of 32 x 32; 32 rows a stage, four stages in LDS.  While a stage's fragments are
-// multiplied,
+// 2 x TILE / 64 waves of TILE / 64 x 2 MFMA tiles of 32 x 32; 32 rows a stage, four stages in LDS.
+// While a stage's fragments are multiplied,
 //   the fragments of the next half stage are read (the next stage's first half too: its writes are a barrier back),
 //   the stage after the next goes from registers through the conversion into its slot of LDS, and
 //   each of those registers is requested again from two stages further on (there are two sets of them: one stage of 32 rows
@@ -203,10 +203,11 @@ __global__ __launch_bounds__(kTnThreads, 2) void gemm_tn_ckpt_kernel(const Args 
 // Conversions, address arithmetic and the bias are what the matrix pipe waits for (counted: of 75 M issue cycles of the first
 // version with one wave a SIMD, the MFMAs took 39 M and other vector instructions 23 M, one after the other); hence two waves
 // a SIMD, constant LDS addresses and buffer loads.
-// 102400 rows, 1024 x 768, bias and join included: int8 164 us, e4m3 (whose conversion is one instruction for two values) 154 us,
-// 0.98 and 1.05 PFLOP/s; an 8192^3 bf16 library product runs at 1.25.  The loop alone is at 1.36: writing every CU's 256 KB of
-// accumulators as partial products and joining them takes the other 25 us.  Consecutive row ranges and tiles on one XCD: 164 us,
-// 184 dealt round (102400 rows, 384 x 384: 54 / 70).
+// 102400 rows, 1024 x 768, bias and join included: int8 168 us, e4m3 (whose conversion is one instruction for two values) 159 us,
+// 0.96 and 1.01 PFLOP/s; an 8192^3 bf16 library product runs at 1.25.  Another 102400 rows add 140 and 130 us (1.15 and 1.24
+// PFLOP/s); what does not grow with the rows, the partial products (256 KB a CU) and their join among it, is about 28 us.
+// Consecutive row ranges and tiles on one XCD: 175 us, 184 dealt round (102400 rows, 384 x 384: 55 / 70).  The large tile spills
+// a few registers: 24 bytes a lane, 76 and 80 through a mask; two of them are read back in each stage of the int8 form.
 // Columns past M: the last chunk of 8 columns is read at M - 8, so that every load is whole and inside; its columns then
 // overlap the chunk before, both give the same sums, and both are written.  Columns past N lie in the checkpoint's padding or
 // are read from its last block; their sums are dropped.
@@ -530,7 +531,7 @@ Plan plan(int64_t rows, int M, int N, int tile) {
     // Row ranges: more of them shorten everybody's loop (32 rows take 0.35 us, 0.75 us with the large tile and all CUs at work),
     // but two or more need the join (6 us for its launch and what it waits for), and each writes and reads back a partial product
     // (0.08 us + 1.1 us for a million elements).  The cheapest number, at least four steps each, at most one round of workgroups;
-    // one where that is cheaper (512 rows, 1024 x 768: 11.5 us, 17.0 with two ranges).
+    // one where that is cheaper (512 rows, 1024 x 768: 11.5 us, 16.7 with two ranges).
     const int64_t steps = (rows + bk - 1) / bk, round = (tile == 256 ? 256 : 512) / tiles;
     const double step = tile == 256 ? 0.75 : 0.35, range = 0.08 + 1.1e-6 * M * N;
     int64_t splits = (int64_t)(sqrt((double)steps * step / range) + 0.5);
