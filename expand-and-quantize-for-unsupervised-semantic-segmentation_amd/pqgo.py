@@ -205,7 +205,7 @@ class _HeadFunction(torch.autograd.Function):
     ``keep`` "int8" / "e4m3": that pair is kept in 8 bits (``native.ckpt_pack``, signs kept, so that the ReLU's mask is exact)
     and the weight gradients are taken straight from the codes, the mask and both biases' sums on the way
     (``native.gemm_tn_ckpt``).  The biases then sum the bf16 rows that the products use too: one pass over the gradient less,
-    and each row's rounding (2^-9 of its value) is as often up as down."""
+    and each row's rounding (at most 2^-8 of its value) is as often up as down."""
 
     @staticmethod
     def forward(ctx, rows, w1, b1, w2a, b2a, w2b, b2b, keep="none"):
