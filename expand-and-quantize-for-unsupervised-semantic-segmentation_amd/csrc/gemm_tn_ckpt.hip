@@ -203,11 +203,11 @@ __global__ __launch_bounds__(kTnThreads, 2) void gemm_tn_ckpt_kernel(const Args 
 // Conversions, address arithmetic and the bias are what the matrix pipe waits for (counted: of 75 M issue cycles of the first
 // version with one wave a SIMD, the MFMAs took 39 M and other vector instructions 23 M, one after the other); hence two waves
 // a SIMD, constant LDS addresses and buffer loads.
-// 102400 rows, 1024 x 768, bias and join included: int8 168 us, e4m3 (whose conversion is one instruction for two values) 159 us,
-// 0.96 and 1.01 PFLOP/s; an 8192^3 bf16 library product runs at 1.25.  Another 102400 rows add 140 and 130 us (1.15 and 1.24
-// PFLOP/s); what does not grow with the rows, the partial products (256 KB a CU) and their join among it, is about 28 us.
+// 102400 rows, 1024 x 768, bias and join included: int8 170 us, e4m3 (whose conversion is one instruction for two values) 159 us,
+// 0.95 and 1.01 PFLOP/s; an 8192^3 bf16 library product runs at 1.25.  Another 102400 rows add 130 and 128 us (1.24 and 1.26
+// PFLOP/s); what does not grow with the rows, the partial products (256 KB a CU) and their join among it, is 30 to 40 us.
 // Consecutive row ranges and tiles on one XCD: 175 us, 184 dealt round (102400 rows, 384 x 384: 55 / 70).  The large tile spills
-// a few registers: 24 bytes a lane, 76 and 80 through a mask; two of them are read back in each stage of the int8 form.
+// a few registers, 24 bytes a lane; two of them are read back in each stage of the int8 form.
 // Columns past M: the last chunk of 8 columns is read at M - 8, so that every load is whole and inside; its columns then
 // overlap the chunk before, both give the same sums, and both are written.  Columns past N lie in the checkpoint's padding or
 // are read from its last block; their sums are dropped.
@@ -379,11 +379,14 @@ __global__ __launch_bounds__(2 * TILE, 2) void gemm_tn_ckpt_tile_kernel(const Ar
 #pragma unroll
             for (int i = ks == 0 ? 0 : BP; i < BP; ++i) { store_b(SET, i, S2); load_b(SET, i); }
             multiply(ks);
-            // the order wanted: behind every MFMA two fragment reads, conversions, and further on the stores and requests
+            // the order wanted: behind every MFMA some fragment reads, conversions, and further on the stores and requests.  Three
+            // reads against two (102400 rows, us): int8 1024 x 768 169 / 172, 384 x 384 52 / 54, e4m3 384 x 384 49 / 50; two in
+            // the large e4m3 tile, which is short of registers: 1024 x 768 160 / 172
+            constexpr int READS = E4M3 && TILE == 256 ? 2 : 3;
 #pragma unroll
             for (int i = 0; i < WM * WNW; ++i) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);            // MFMA
-                if (i < WM + WNW) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);   // LDS reads
+                if (i * READS < 2 * (WM + WNW)) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);   // LDS reads
                 __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);            // VALU
                 if (i >= WM * WNW / 2) {
                     __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);        // LDS write
@@ -547,12 +550,16 @@ Plan plan(int64_t rows, int M, int N, int tile) {
     return p;
 }
 
-int tile_of(int64_t rows, int M, int N) {
+// The large tile reads half as much LDS for a product, which pays where every CU has a long way to go (2e10 products) and little of
+// the tile lies outside: more than three small tiles to a large one.  Measured (us, int8; 128 against 256):
+//   25088 x 1024 x 768 60 / 63, 51200 x 1024 x 768 102 / 92, 102400 x 1024 x 768 204 / 169, 102400 x 512 x 512 77 / 73
+//   three to one: 102400 x 1024 x 384 113 / 113, 102400 x 384 x 768 85 / 90;  fewer: 640 x 384 72 / 85, 384 x 384 52 / 62
+// Through a mask it runs out of registers: 102400 rows, 768 x 768 188 / 194, 640 x 384 90 / 118, 384 x 384 59 / 82, 1024 x 768
+// 247 / 242, and only long and narrow products would gain (1024 x 200 104 / 92); it has no such form.
+int tile_of(int64_t rows, int M, int N, bool mask) {
     if (M < 8) return 0;
-    // Measured (us, int8; 128 against 256): 25088 x 1024 x 768 65 / 63, 12544 x 1024 x 768 42 / 44, 102400 x 384 x 384 57 / 68,
-    // 102400 x 1024 x 768 217 / 164, 1024 x 1024 x 768 18 / 25: the large tile, which reads half as much LDS
-    // for a product, pays where every CU has a long way to go.
-    return (double)rows * M * N >= 2e10 && M > 128 && N > 128 ? 256 : 128;
+    const int64_t small = (int64_t)((M + 127) / 128) * ((N + 127) / 128), large = (int64_t)((M + 255) / 256) * ((N + 255) / 256);
+    return !mask && (double)rows * M * N >= 2e10 && small > 3 * large ? 256 : 128;
 }
 
 // partial products and, behind them, partial bias sums; nothing where one row range writes the results
@@ -564,9 +571,14 @@ size_t workspace(const Plan& p, int M, int N) {
 
 extern "C" size_t equss_gemm_tn_ckpt_workspace_bytes(int64_t rows, int M, int N) {
     if (rows < 0 || M <= 0 || N <= 0) return 0;
-    // (the narrow kernel stands in where leading dimensions are too long for the others)
-    const size_t a = workspace(plan(rows, M, N, tile_of(rows, M, N)), M, N), b = workspace(plan(rows, M, N, 0), M, N);
-    return a > b ? a : b;
+    // with a mask or without, and the narrow kernel, which stands in where leading dimensions are too long for the others
+    const int tiles[3] = {tile_of(rows, M, N, false), tile_of(rows, M, N, true), 0};
+    size_t most = 0;
+    for (int tile : tiles) {
+        const size_t one = workspace(plan(rows, M, N, tile), M, N);
+        if (one > most) most = one;
+    }
+    return most;
 }
 
 extern "C" int equss_gemm_tn_ckpt(const void* a, int64_t lda, const void* codes, int64_t ld_codes, const void* scales, int64_t ld_scales,
@@ -586,7 +598,7 @@ extern "C" int equss_gemm_tn_ckpt(const void* a, int64_t lda, const void* codes,
         return equss::fail(EQUSS_E_ALIGN, "equss_gemm_tn_ckpt: mask codes 16-byte aligned with a leading dimension that is a multiple of 32 "
                            "and holds %d", g.mpad);
     const size_t need = equss_gemm_tn_ckpt_workspace_bytes(rows, M, N);
-    Plan p = plan(rows, M, N, tile_of(rows, M, N));
+    Plan p = plan(rows, M, N, tile_of(rows, M, N, relu_codes != nullptr));
     if (p.tile && !(offsets_fit(p, lda * 2) && offsets_fit(p, ld_codes) && offsets_fit(p, ld_scales) && offsets_fit(p, relu_codes ? ld_relu : 0)))
         p = plan(rows, M, N, 0);
     if (need > 0 && (!workspace_ptr || workspace_bytes < need || ((uintptr_t)workspace_ptr % 16) != 0))
@@ -615,12 +627,9 @@ extern "C" int equss_gemm_tn_ckpt(const void* a, int64_t lda, const void* codes,
             return equss::fail(EQUSS_E_UNSUPPORTED, "equss_gemm_tn_ckpt: %d bytes of LDS", lds);                               \
         hipLaunchKernelGGL((gemm_tn_ckpt_tile_kernel<E, K, T>), grid, dim3(2 * T), lds, s, g);                                 \
     } while (0)
-#define EQUSS_TN_FORM(T)                                                                                                       \
-    if (e) { if (relu_codes) EQUSS_TN_TILE(true, true, T); else EQUSS_TN_TILE(true, false, T); }                               \
-    else { if (relu_codes) EQUSS_TN_TILE(false, true, T); else EQUSS_TN_TILE(false, false, T); }
-        if (p.tile == 256) { EQUSS_TN_FORM(256) }
-        else { EQUSS_TN_FORM(128) }
-#undef EQUSS_TN_FORM
+        if (p.tile == 256) { if (e) EQUSS_TN_TILE(true, false, 256); else EQUSS_TN_TILE(false, false, 256); }
+        else if (relu_codes) { if (e) EQUSS_TN_TILE(true, true, 128); else EQUSS_TN_TILE(false, true, 128); }
+        else { if (e) EQUSS_TN_TILE(true, false, 128); else EQUSS_TN_TILE(false, false, 128); }
 #undef EQUSS_TN_TILE
     } else {
         const dim3 grid((unsigned)blocks), block(kTnThreads);

@@ -355,3 +355,22 @@ def test_offsets_past_32_bits(native, dev):
     last = native.ActCheckpoint(kept.codes[-tail:].contiguous(), kept.scales[-tail:].contiguous(), width)
     want, _ = native.pq_st_backward_ckpt(last, books, idx[:, -tail:], g[-tail:], zero, 0.25, 1.0)
     assert torch.equal(gz[-tail:], want) and not bool(gz[:-tail].any()) and not bool(gb.any())
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("rows,m,n", [(30011, 1001, 701), (2001, 4001, 2601), (25000, 1024, 800), (56003, 1000, 384), (21011, 2500, 391)])
+def test_weight_gradient_is_exact_where_the_work_is_large(rows, m, n, fmt, native, dev):
+    """More than 2e10 products, where the tiles of 256 stand in: several row ranges and one, edges inside a tile, the bias with and
+    without; shapes that lie badly in them; the same through a mask.  Whole numbers below 2^24, exact in fp32 in any order."""
+    g = torch.Generator().manual_seed(rows)
+    a = torch.randint(-2, 3, (rows, m), generator=g).to(torch.bfloat16)
+    v, kept = whole_numbers(rows, n, fmt, 5, dev, native)
+    assert rows * m * n >= 2e10 and rows * 2 * 60 < 2 ** 24
+    want, sums = a.float().t() @ v.float(), a.float().sum(0)
+    assert torch.equal(native.gemm_tn_ckpt(a.to(dev), kept).cpu(), want)
+    dw, db = native.gemm_tn_ckpt(a.to(dev), kept, want_bias=True)
+    assert torch.equal(dw.cpu(), want) and torch.equal(db.cpu(), sums)
+    h = torch.relu(torch.randn(rows, m, generator=g))
+    dw, db = native.gemm_tn_ckpt(a.to(dev), kept, relu=native.ckpt_pack(h.to(dev), fmt, keep_sign=True), want_bias=True)
+    am = a.float() * (h > 0)
+    assert torch.equal(dw.cpu(), am.t() @ v.float()) and torch.equal(db.cpu(), am.sum(0))
