@@ -374,3 +374,13 @@ def test_weight_gradient_is_exact_where_the_work_is_large(rows, m, n, fmt, nativ
     dw, db = native.gemm_tn_ckpt(a.to(dev), kept, relu=native.ckpt_pack(h.to(dev), fmt, keep_sign=True), want_bias=True)
     am = a.float() * (h > 0)
     assert torch.equal(dw.cpu(), am.t() @ v.float()) and torch.equal(db.cpu(), am.sum(0))
+
+
+@pytest.mark.parametrize("n,num_pq,k,d,fmt", [(70003, 8, 100, 128, "int8"), (140001, 8, 256, 64, "e4m3")])
+def test_quantiser_backward_matches_the_formula_where_the_chip_is_full(n, num_pq, k, d, fmt, native, dev):
+    """Enough rows for tiles of 64 everywhere (rows / 64 times sub-spaces times lanes a row, 2^18 or more); bounds as above."""
+    assert (n + 63) // 64 * num_pq * (d // 4) >= 2 ** 18
+    z, books, idx, g_zq, g_vq = pq_case(n, num_pq, k, d, fmt, n, skew=2.0)
+    kept = native.ckpt_pack(z.to(dev), fmt)
+    want = pq_formula(native.ckpt_unpack(kept).cpu(), books, idx, g_zq, g_vq, 0.25, 1.5)
+    check_pq(native.pq_st_backward_ckpt(kept, books.to(dev), idx.to(dev), g_zq.to(dev), g_vq.to(dev), 0.25, 1.5), want, (n, num_pq, k, d, fmt))

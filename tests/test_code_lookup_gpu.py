@@ -130,3 +130,16 @@ def test_lookup_calls_in_replayed_graphs(native, dev):
             assert all(torch.equal(x, y) for x, y in zip(h, want)), i
         native.code_lookup_grad(g[:3000], idx[:, :3000], k)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("rows,num_pq,k,d", [(70003, 8, 256, 128), (70003, 40, 20, 28), (70003, 4, 2100, 300)])
+def test_lookup_gradient_is_exact_where_the_chip_is_full(rows, num_pq, k, d, native, dev):
+    """Enough rows for tiles of 64 everywhere, one row in flight a group: rows / 64 of them times sub-spaces times lanes a row, 2^18 or more.
+    Whole numbers below 2^24 add exactly in any order."""
+    assert (rows + 63) // 64 * num_pq * min(64, (d + 3) // 4) >= 2 ** 18 and rows * 8 * 4 < 2 ** 24
+    g = torch.randint(-8, 9, (rows, num_pq * d), generator=torch.Generator().manual_seed(rows + d)).to(F32)
+    for skew, bad in ((2.0, 0.02), (1e9, 0.3)):
+        idx = indices(num_pq, rows, k, 3, skew, bad)
+        want = plain_grad(g, idx, k, 4.0).to(F32)
+        got = native.code_lookup_grad(g.to(dev), idx.to(dev), k, 4.0)
+        assert torch.equal(got.cpu(), want), skew
