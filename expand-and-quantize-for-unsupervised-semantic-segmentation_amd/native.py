@@ -346,17 +346,22 @@ def layernorm_bf16(x, gamma, beta, eps=1e-6, tokens_per_image=0, out=None, want_
 
 
 def gemm_bf16(a, w, bias, epilogue, out=None):
-    """out = epilogue(a @ w.T + bias); a (M,K) bf16, w (N,K) bf16, bias (N,) fp32 or None."""
+    """out = epilogue(a @ w.T + bias); a (M,K) bf16, w (N,K) bf16, bias (N,) fp32 or None.  Operands whose columns are not
+    consecutive are copied."""
     lib = load_library()
     _need_cuda(a, w, bias)
     m, k = a.shape
     n = w.shape[0]
+    a, lda = _row_major(a)
+    w, ldw = _row_major(w)
+    if out is not None and out.stride(1) != 1:
+        raise ValueError("gemm_bf16: the columns of `out` must be consecutive")
     if out is None:
         dt = torch.float32 if epilogue in (EPI_F32, EPI_RESID_F32) else torch.bfloat16
         if epilogue == EPI_RESID_F32:
             raise ValueError("the residual epilogue accumulates into `out`; pass it")
         out = torch.empty((m, n), dtype=dt, device=a.device)
-    rc = lib.equss_gemm_bf16(_ptr(a), a.stride(0), _ptr(w), w.stride(0), _ptr(bias), _ptr(out), out.stride(0),
+    rc = lib.equss_gemm_bf16(_ptr(a), lda, _ptr(w), ldw, _ptr(bias), _ptr(out), out.stride(0),
                              m, n, k, int(epilogue), _stream(a))
     _check(rc, "equss_gemm_bf16")
     return out

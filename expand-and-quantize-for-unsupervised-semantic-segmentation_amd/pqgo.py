@@ -233,7 +233,7 @@ class _HeadFunction(torch.autograd.Function):
         c = w_cat.shape[1] // 2
         s1, s2a, s2b = ctx.shapes
         kept = native.ActCheckpoint(codes, scales, 2 * c)
-        g_bf = g.to(torch.bfloat16)
+        g_bf = g.to(torch.bfloat16).contiguous()                             # (one image: its rows may lie by channels)
         dw_cat, db = native.gemm_tn_ckpt(g_bf, kept, want_bias=True)         # (D, 2C) = [dW1 | dW2b]
         w2b_t = w_cat[:, c:].t().contiguous()
         d_h = native.gemm_bf16(g_bf, w2b_t, None, native.EPI_BF16) if c % 128 == 0 and w_cat.shape[0] % 128 == 0 else torch.mm(g_bf, w2b_t.t())
@@ -248,7 +248,7 @@ class _HeadFunction(torch.autograd.Function):
         c = fh.shape[1] // 2
         d = w_cat.shape[0]
         s1, s2a, s2b = ctx.shapes
-        g_bf = g.to(torch.bfloat16)
+        g_bf = g.to(torch.bfloat16).contiguous()                         # (one image: its rows may lie by channels)
         if _HeadFunction.native_backward and c % 128 == 0 and d % 128 == 0:
             # dW = g^T f sums over batch * tokens: the split-K transposed-operand kernel; d_pre is an ordinary A W^T GEMM
             dw_cat = native.gemm_tn_bf16(g_bf, fh)                   # (D, 2C) = [dW1 | dW2b]

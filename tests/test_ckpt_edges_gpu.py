@@ -1,0 +1,59 @@
+"""The checkpointed training pass and its operators where layouts, missing gradients and the ends of the number formats meet
+them."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F64 = torch.float64
+U = 2.0 ** -24
+
+
+@pytest.mark.parametrize("keep", ["none", "int8", "e4m3"])
+def test_head_gradients_of_one_image_whose_gradient_lies_by_channels(keep, pkg, dev):
+    """With one image, the rows of an NCHW-contiguous gradient have a column stride of h w and a row stride of 1.  Whole numbers
+    of at most 256 throughout (sums below 2^24): every product and sum is exact, so both layouts give equal bits."""
+    h, w, c, d = 9, 7, 128, 256
+    g0 = torch.Generator().manual_seed(11)
+
+    def whole(*shape):
+        return torch.randint(-1, 2, shape, generator=g0).float().to(dev)
+
+    rows = whole(h * w, c)
+    par = [whole(*s).requires_grad_(True) for s in ((d, c, 1, 1), (d,), (c, c, 1, 1), (c,), (d, c, 1, 1), (d,))]
+    grad = whole(1, d, h, w)
+    by_rows = grad.permute(0, 2, 3, 1).reshape(-1, d).contiguous()
+    by_channels = grad.permute(0, 2, 3, 1).reshape(-1, d)
+    assert by_channels.stride() == (1, h * w) and torch.equal(by_rows, by_channels)
+    code = pkg.pqgo._HeadFunction.apply(rows, *par, keep)
+    want = torch.autograd.grad(code, par, by_rows, retain_graph=True)
+    got = torch.autograd.grad(code, par, by_channels)
+    assert all(bool(t.any()) for t in want) and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_row_products_take_operands_of_any_strides(native, dev):
+    """native.gemm_bf16 of transposed, column-strided and one-row operands; an output it cannot write is refused."""
+    g = torch.Generator().manual_seed(12)
+    a = torch.randint(-2, 3, (256, 128), generator=g).to(torch.bfloat16).to(dev)
+    w = torch.randint(-2, 3, (128, 128), generator=g).to(torch.bfloat16).to(dev)
+    want = (a.cpu().to(F64) @ w.cpu().to(F64).t()).to(torch.bfloat16)
+    for x in (a, a.t().contiguous().t(), a.repeat_interleave(2, dim=1)[:, ::2]):
+        for y in (w, w.t().contiguous().t(), w.repeat_interleave(2, dim=1)[:, ::2]):
+            assert torch.equal(native.gemm_bf16(x, y, None, native.EPI_BF16).cpu(), want)
+    one = a.t().contiguous().t()[:1]
+    assert torch.equal(native.gemm_bf16(one, w, None, native.EPI_BF16).cpu(), want[:1])
+    with pytest.raises(ValueError, match="out"):
+        native.gemm_bf16(a, w, None, native.EPI_BF16, out=torch.empty(128, 256, dtype=torch.bfloat16, device=dev).t())
+
+
+@pytest.mark.parametrize("keep", ["none", "int8", "e4m3"])
+def test_training_step_of_one_image(keep, pkg, dev):
+    cfg = pkg.configs.pqgo_config(need_initialized="none", drop_prob=0.0, activation_checkpoint=keep)
+    m = pkg.build_model(cfg)
+    m.load_state_dict(pkg.synth.synth_pqgo_state(cfg, seed=1234), strict=True)
+    m = m.to(dev).train()
+    img = pkg.synth.synth_images(1, 64, 64, seed=71).to(dev)
+    label = pkg.synth.synth_labels(1, 64, 64, cfg["num_classes"], seed=71).to(dev)
+    total, _out, _preds, _vq = m(img=img, aug_img=img, label=label, img_pos=img.flip(3), it=0)
+    total.backward()
+    assert all(p.grad is not None and bool(torch.isfinite(p.grad).all()) for p in m.parameters() if p.requires_grad)
