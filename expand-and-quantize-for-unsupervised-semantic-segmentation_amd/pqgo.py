@@ -324,18 +324,16 @@ class _PQStraightThrough(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g_zq, g_vq, _g_idx):
         num_pq, k, d, beta, book = ctx.meta
+        if g_vq is None:
+            g_vq = torch.zeros((), dtype=torch.float32, device=ctx.saved_tensors[0].device)
         if ctx.kept:
             codes, scales, books, idx = ctx.saved_tensors
-            if g_vq is None:
-                g_vq = torch.zeros((), dtype=torch.float32, device=codes.device)
             g_rows, g_books = native.pq_st_backward_ckpt(native.ActCheckpoint(codes, scales, num_pq * d), books, idx, g_zq, g_vq, beta, book,
                                                          want_rows=ctx.needs_input_grad[0], want_books=ctx.needs_input_grad[1])
             return g_rows, g_books, None, None, None
         rows, emb, idx = ctx.saved_tensors
         n = rows.shape[0]
         if _PQStraightThrough.hip_backward:
-            if g_vq is None:
-                g_vq = torch.zeros((), dtype=torch.float32, device=rows.device)
             g_rows, g_books = native.pq_st_backward(rows, emb, idx, g_zq, g_vq, beta, book, k, d,
                                                     want_rows=ctx.needs_input_grad[0], want_books=ctx.needs_input_grad[1])
             return g_rows, g_books, None, None, None

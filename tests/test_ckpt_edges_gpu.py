@@ -57,3 +57,28 @@ def test_training_step_of_one_image(keep, pkg, dev):
     total, _out, _preds, _vq = m(img=img, aug_img=img, label=label, img_pos=img.flip(3), it=0)
     total.backward()
     assert all(p.grad is not None and bool(torch.isfinite(p.grad).all()) for p in m.parameters() if p.requires_grad)
+
+
+@pytest.mark.parametrize("keep", ["none", "int8"])
+@pytest.mark.parametrize("closed_form", [False, True])
+def test_quantiser_gradient_of_the_quantised_output_alone(closed_form, keep, pkg, native, dev, monkeypatch):
+    """A loss that reaches the quantiser through zq only, and one through vq only, in every branch of the backward, against the
+    formula in fp64: g_z = (g - zn <zn, g>) / |z| at the z that the branch keeps (64 u of |g| / |z|: the norm's sum, two products
+    and the projection are below 32 roundings deep)."""
+    monkeypatch.setattr(pkg.pqgo._PQStraightThrough, "hip_backward", not closed_form)
+    torch.manual_seed(7)
+    n, p, k, d = 300, 2, 32, 32
+    z = torch.randn(n, p * d, device=dev, requires_grad=True)
+    books = (torch.randn(p, k, d, device=dev) * 0.2).requires_grad_(True)
+    g = torch.randn(n, p * d, device=dev)
+    zq, vq, _ = pkg.pqgo._PQStraightThrough.apply(z, books, 0.25, 1.0, keep)
+    gz, gb = torch.autograd.grad(zq, [z, books], g, retain_graph=True)
+    zk = z.detach() if keep == "none" else native.ckpt_unpack(native.ckpt_pack(z.detach(), keep))
+    z3, g3 = zk.cpu().to(F64).reshape(n, p, d), g.cpu().to(F64).reshape(n, p, d)
+    norm = z3.norm(dim=-1, keepdim=True)
+    zn = z3 / norm
+    want = (g3 - zn * (zn * g3).sum(-1, keepdim=True)) / norm
+    assert bool(((gz.cpu().to(F64).reshape(n, p, d) - want).abs() <= 64 * U * g3.norm(dim=-1, keepdim=True) / norm).all())
+    assert not bool(gb.any())
+    gz, gb = torch.autograd.grad(vq, [z, books])
+    assert bool(gz.any()) and bool(gb.any())
