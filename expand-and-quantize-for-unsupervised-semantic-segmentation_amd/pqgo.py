@@ -360,13 +360,19 @@ class _PQStraightThrough(torch.autograd.Function):
 
 class _CodeLookup(torch.autograd.Function):
     """out = scale * books[p, idx[p, r]]; linear in the books, and so is its gradient in its own input: each is the other's
-    backward, to any order."""
+    backward, to any order, and carries tangents as it carries values."""
 
     @staticmethod
     def forward(ctx, idx, books, scale):
         ctx.save_for_backward(idx)
+        ctx.save_for_forward(idx)
         ctx.meta = (books.shape[1], scale, books.dtype)
         return native.code_lookup(idx, books, scale)
+
+    @staticmethod
+    def jvp(ctx, _idx, t, _scale):
+        (idx,) = ctx.saved_tensors
+        return _CodeLookup.apply(idx, t, ctx.meta[1])
 
     @staticmethod
     def backward(ctx, g):
@@ -379,20 +385,26 @@ class _CodeLookupGrad(torch.autograd.Function):
     @staticmethod
     def forward(ctx, idx, g, k, scale):
         ctx.save_for_backward(idx)
-        ctx.meta = (scale, g.dtype)
+        ctx.save_for_forward(idx)
+        ctx.meta = (k, scale, g.dtype)
         return native.code_lookup_grad(g, idx, k, scale)
+
+    @staticmethod
+    def jvp(ctx, _idx, t, _k, _scale):
+        (idx,) = ctx.saved_tensors
+        return _CodeLookupGrad.apply(idx, t, *ctx.meta[:2])
 
     @staticmethod
     def backward(ctx, gg):
         (idx,) = ctx.saved_tensors
-        scale, dtype = ctx.meta
+        _, scale, dtype = ctx.meta
         return None, _CodeLookup.apply(idx, gg, scale).to(dtype), None, None
 
 
 def code_lookup(idx, books, scale=1.0):
     """Codewords by their indices (the gather of dino_pqgo.py:659-663 on its own): idx (num_pq, rows) integer, any strides; books
     (num_pq, K, d) -> (rows, num_pq*d) = scale * books[p, idx[p, r]], zeros where an index lies outside [0, K).  Differentiable
-    in the books; the gradient sums every codeword's rows in a fixed order."""
+    in the books, backward and forward; the gradient sums every codeword's rows in a fixed order."""
     return _CodeLookup.apply(idx, books, float(scale))
 
 
