@@ -159,9 +159,20 @@ __global__ __launch_bounds__(kThreads) void ckpt_pack_kernel(const typename Elem
                 }
             }
         }
+        if (lost) {
+#pragma unroll
+            for (int h = 0; h < V / 4; ++h) {
+                out[h] = 0;
+                if constexpr (KEEP) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        out[h] |= (v[4 * h + i] > 0.f ? (E4M3 ? 0x7fu : 1u) : v[4 * h + i] < 0.f ? 0xffu : 0u) << (8 * i);
+                }
+            }
+        }
         uint8_t* dst = codes + row * ld_codes + col;
-        if constexpr (V == 4) *reinterpret_cast<uint32_t*>(dst) = lost ? 0u : out[0];
-        else *reinterpret_cast<uint2*>(dst) = lost ? make_uint2(0, 0) : make_uint2(out[0], out[V / 4 - 1]);
+        if constexpr (V == 4) *reinterpret_cast<uint32_t*>(dst) = out[0];
+        else *reinterpret_cast<uint2*>(dst) = make_uint2(out[0], out[V / 4 - 1]);
         if ((u & (LANES - 1)) == 0) scales[row * ld_scales + col / equss::kCkptBlock] = (uint8_t)(lost ? equss::kCkptNanByte : k + 127);
     }
 }
@@ -187,7 +198,7 @@ __global__ __launch_bounds__(kThreads) void ckpt_unpack_kernel(const uint8_t* __
             c[0] = w2.x;
             c[V / 4 - 1] = w2.y;
         }
-        const float s = equss::ckpt_scale(scales[row * ld_scales + col / equss::kCkptBlock]);
+        const float s = equss::ckpt_value_scale(scales[row * ld_scales + col / equss::kCkptBlock]);
         float v[V];
 #pragma unroll
         for (int h = 0; h < V / 4; ++h) {

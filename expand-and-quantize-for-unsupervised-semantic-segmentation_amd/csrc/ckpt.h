@@ -11,9 +11,15 @@ namespace equss {
 
 constexpr int kCkptBlock = 32;
 constexpr int kCkptMinExp = -110;      // smallest scale exponent: what is kept, e4m3's subnormals included, is a normal fp32 / bf16
-constexpr int kCkptNanByte = 255;      // scale byte of a block that held an infinity or a NaN: (255 << 23) is inf, times code 0 is NaN
+// Scale byte of a block that held an infinity or a NaN.  Its codes are 0, or, where signs are kept, a code of the value's sign:
+// -1 or 1 in int8, a NaN of that sign in e4m3.  255 << 23 is an infinity, times code 0 a NaN; ckpt_value_scale makes it a NaN
+// whatever the code.  The products (gemm_tn_ckpt.hip) do without that: a lost block is infinities or NaN there.
+constexpr int kCkptNanByte = 255;
 
 __device__ __forceinline__ float ckpt_scale(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
+__device__ __forceinline__ float ckpt_value_scale(uint32_t byte) {
+    return __builtin_bit_cast(float, byte == (uint32_t)kCkptNanByte ? 0x7fc00000u : byte << 23);
+}
 
 // code number I (0..3) of a dword, before scaling
 template <bool E4M3>

@@ -51,7 +51,7 @@ struct PqOp {
     }
     __device__ __forceinline__ f32x4 value(Row& r) const {
         const float s = a.g_vq[0] * a.inv_count, bs = a.beta * s;
-        const f32x4 z = equss::ckpt_decode4<E4M3>(r.q) * equss::ckpt_scale(r.scale);
+        const f32x4 z = equss::ckpt_decode4<E4M3>(r.q) * equss::ckpt_value_scale(r.scale);
         const float len = sqrtf(equss::lanes_sum<LPR>(z.x * z.x + z.y * z.y + z.z * z.z + z.w * z.w));
         const bool tiny = len < 1e-12f;
         const float inv = 1.f / (tiny ? 1e-12f : len);

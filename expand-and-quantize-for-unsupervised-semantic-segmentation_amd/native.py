@@ -758,7 +758,8 @@ def _at(t):
 def ckpt_pack(x, fmt="int8", keep_sign=False):
     """x (rows, width) fp32 / bf16 / fp16 -> ActCheckpoint in ``fmt`` "int8" or "e4m3": one byte a value and one for 32
     consecutive channels.  ``keep_sign``: a value other than zero never becomes zero, so that ``code > 0`` is the mask of a
-    ReLU whose result is kept (see equss_ckpt_pack in the header for the rounding)."""
+    ReLU whose result is kept, also where a block holds an infinity or a NaN (see equss_ckpt_pack in the header for the
+    rounding)."""
     if not x.is_cuda:
         _need_cuda(x)
     if fmt not in CKPT_FORMATS:

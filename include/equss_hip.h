@@ -417,9 +417,10 @@ int equss_code_sums(const float* z, int64_t ld_z, const int64_t* idx, float* sum
  * largest magnitude A, the scale is 2^k with the smallest integer k >= -110 for which A 2^-k, rounded to the format, does not
  * pass its largest value (int8: 127, e4m3: 448); a code is x 2^-k rounded to nearest even, off by half a step of the format at
  * most.  Nothing saturates, and every kept value is exact in bf16 and fp32.  A block that holds an infinity or a NaN gets scale
- * byte 255 and codes 0 and reads back as NaN throughout.
+ * byte 255 and codes 0 and reads back as NaN throughout (in equss_gemm_tn_ckpt: as infinities or NaN).
  *   keep_sign != 0: a value other than zero that would round to zero becomes the smallest code of its sign instead (off by less
- *            than one such step), so that "code > 0" is the mask of a ReLU whose result is kept
+ *            than one such step), so that "code > 0" is the mask of a ReLU whose result is kept.  That holds in a block of scale
+ *            byte 255 too, whose codes are then -1, 0 and 1 (int8) or 0 and the two NaN (e4m3) by their values' signs, a NaN's 0
  *   x / out  (rows, width), type EQUSS_F32 / _BF16 / _F16, unit column stride, leading dimension in elements, any alignment
  *   codes    (rows, ld_codes) bytes out / in, 16-byte aligned, ld_codes a multiple of 32, >= width rounded up to 32 (the padding
  *            is written as zero codes); scales (rows, ld_scales) bytes, one for each block of 32

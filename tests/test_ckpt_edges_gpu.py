@@ -82,3 +82,50 @@ def test_quantiser_gradient_of_the_quantised_output_alone(closed_form, keep, pkg
     assert not bool(gb.any())
     gz, gb = torch.autograd.grad(vq, [z, books])
     assert bool(gz.any()) and bool(gb.any())
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_mask_of_a_block_that_holds_an_infinity_or_a_nan(fmt, native, dev):
+    """Signs are kept there too: a place counts where its value is positive, an infinity among them, and the block still reads
+    back as NaN throughout.  What lies outside such blocks is not touched."""
+    g = torch.Generator().manual_seed(13)
+    rows, m, n = 40, 96, 64
+    h = torch.randn(rows, m, generator=g)
+    h[3, 5], h[7, 40], h[9, 70], h[11, 71] = float("inf"), -float("inf"), float("nan"), float("inf")
+    h[3, 6] = 0.0
+    h[11, 64:71] = torch.tensor([1e-45, -1e-45, 0.0, -0.0, 3e38, -3e38, float("nan")])
+    kept = native.ckpt_pack(h.to(dev), fmt, keep_sign=True)
+    codes = kept.codes.view(torch.int8).cpu()
+    assert torch.equal(codes > 0, h > 0) and torch.equal(codes < 0, h < 0)
+    lost = (~torch.isfinite(h)).reshape(rows, -1, 32).any(-1).repeat_interleave(32, 1)
+    assert bool((kept.scales.cpu()[lost[:, ::32]] == 255).all())
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        back = native.ckpt_unpack(kept, dtype).cpu()
+        assert bool(torch.isnan(back[lost]).all()) and not bool(torch.isnan(back[~lost]).any())
+    a = torch.randint(-2, 3, (rows, m), generator=g).to(torch.bfloat16)
+    v = torch.randint(-15, 16, (rows, n), generator=g).float()
+    am = a.to(F64) * (h > 0)
+    vk = native.ckpt_pack(v.to(dev), fmt)
+    dw, db = native.gemm_tn_ckpt(a.to(dev), vk, relu=kept, want_bias=True)
+    assert torch.equal(dw.cpu(), (am.t() @ v.to(F64)).float()) and torch.equal(db.cpu(), am.sum(0).float())
+    dw = native.gemm_tn_ckpt(a[:, :5].to(dev), vk, relu=native.ckpt_pack(h[:, :5].to(dev), fmt, keep_sign=True))     # narrow form
+    assert torch.equal(dw.cpu(), (am[:, :5].t() @ v.to(F64)).float())
+    # as the kept input of the layer: its columns of the product are not finite, the others are
+    spoilt = native.gemm_tn_ckpt(torch.ones(rows, 16, dtype=torch.bfloat16, device=dev), kept).cpu()
+    cols = lost.any(0)
+    assert not bool(torch.isfinite(spoilt[:, cols]).any()) and bool(torch.isfinite(spoilt[:, ~cols]).all())
+
+
+def test_quantiser_backward_shows_a_lost_block_throughout_its_codeword(native, dev):
+    """A block that lost its values spoils its sub-space of its row and the codeword's gradient, all d columns, nothing else."""
+    n, p, k, d = 50, 2, 8, 64
+    z = torch.randn(n, p * d, generator=torch.Generator().manual_seed(14))
+    z[20, 70] = float("inf")
+    books, idx = torch.randn(p, k, d), torch.arange(n).remainder(k).repeat(p, 1)
+    for keep in (False, True):
+        for fmt in ("int8", "e4m3"):
+            kept = native.ckpt_pack(z.to(dev), fmt, keep_sign=keep)
+            gz, gb = native.pq_st_backward_ckpt(kept, books.to(dev), idx.to(dev), torch.randn(n, p * d, device=dev), torch.ones((), device=dev), 0.25, 1.0)
+            bad_z, bad_b = torch.isnan(gz).cpu(), torch.isnan(gb).cpu()
+            assert bool(bad_z[20, d:].all()) and int(bad_z.sum()) == d
+            assert bool(bad_b[1, 20 % k].all()) and int(bad_b.sum()) == d
