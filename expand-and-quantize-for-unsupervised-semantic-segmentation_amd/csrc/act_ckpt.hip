@@ -7,6 +7,8 @@
 // (int8) or 448 (e4m3).  With e = floor(log2(amax)), amax 2^-(e-6) lies in [64, 128) and amax 2^-(e-8) in [256, 512): the
 // exponent is right as it is unless the mantissa rounds past the end (127.5 up; above 464, the middle between 448 and the 480
 // that e4m3 does not have), where it is one more.  Every code is then off by half a step at most; none saturates.
+// At the top of fp32 and bf16 the raised exponent makes the largest codes 64 or 256 times 2^k = 2^128: an infinity, as rounding
+// to fewer bits has it anywhere (a cap would keep such a value finite at the cost of a whole step).
 #include "ckpt.h"
 
 namespace {

@@ -777,7 +777,9 @@ def ckpt_pack(x, fmt="int8", keep_sign=False):
 
 
 def ckpt_unpack(ckpt, dtype=torch.float32):
-    """The kept values (rows, width) in fp32, bf16 or fp16 (exact in the first two)."""
+    """The kept values (rows, width) in fp32, bf16 or fp16 (exact in the first two).  Magnitudes within 2^-7 (int8) or 2^-5 (e4m3)
+    of 2^128, or of 2^16 where they are read as fp16, may have been rounded up to that and read back as infinities: the lowest
+    number of a type is no filler for what is to be kept."""
     _same_device(ckpt.codes, ckpt.scales)
     if dtype not in _ELEM_TYPES:
         raise ValueError("ckpt_unpack: dtype must be float32, bfloat16 or float16")

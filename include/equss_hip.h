@@ -416,7 +416,10 @@ int equss_code_sums(const float* z, int64_t ld_z, const int64_t* idx, float* sum
  * consecutive channels of a row (the last block of a row may be shorter).  Scale byte b stands for 2^(b - 127).  Of a block with
  * largest magnitude A, the scale is 2^k with the smallest integer k >= -110 for which A 2^-k, rounded to the format, does not
  * pass its largest value (int8: 127, e4m3: 448); a code is x 2^-k rounded to nearest even, off by half a step of the format at
- * most.  Nothing saturates, and every kept value is exact in bf16 and fp32.  A block that holds an infinity or a NaN gets scale
+ * most.  Nothing saturates, and every kept value below 2^128 is exact in bf16 and fp32.  Rounding passes the largest number of a
+ * type where it would in that type too: a magnitude of 2^128 (1 - 2^-7) (int8) or 2^128 (1 - 2^-5) (e4m3) or more may be kept as
+ * 2^128, which is an infinity in fp32, bf16 and the products; of 2^16 (1 - 2^-7) or 2^16 (1 - 2^-5) or more as 2^16, which is
+ * one where it is read as fp16, and exact elsewhere.  The lowest number of a type as a mask's filler is such a value.  A block that holds an infinity or a NaN gets scale
  * byte 255 and codes 0 and reads back as NaN throughout (in equss_gemm_tn_ckpt: as infinities or NaN).
  *   keep_sign != 0: a value other than zero that would round to zero becomes the smallest code of its sign instead (off by less
  *            than one such step), so that "code > 0" is the mask of a ReLU whose result is kept.  That holds in a block of scale

@@ -129,3 +129,29 @@ def test_quantiser_backward_shows_a_lost_block_throughout_its_codeword(native, d
             bad_z, bad_b = torch.isnan(gz).cpu(), torch.isnan(gb).cpu()
             assert bool(bad_z[20, d:].all()) and int(bad_z.sum()) == d
             assert bool(bad_b[1, 20 % k].all()) and int(bad_b.sum()) == d
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_largest_numbers_of_every_type(fmt, native, dev):
+    """A block's largest number decides the scale 2^k: int8 keeps 127 2^(k) up to 127.5 2^k and takes k + 1 from there, e4m3 448 up
+    to 464.  With the raised scale 63.5 (int8) or 248 (e4m3) and more of it round to 64 or 256, i.e. to 2^128 at the top of fp32
+    and bf16 and to 2^16 at the top of fp16; everything below stays finite and within half a step."""
+    raised, up, step = (127.5 / 128, 63.5 / 64, 1 / 64) if fmt == "int8" else (464 / 512, 248 / 256, 16 / 256)
+    for dtype, top in ((torch.float32, 128), (torch.bfloat16, 128), (torch.float16, 16)):
+        largest = torch.finfo(dtype).max
+        x = torch.zeros(6, 32, dtype=F64)
+        x[:, 0] = torch.tensor([largest, -largest, raised * 0.995 * 2.0 ** top, up * 0.95 * 2.0 ** top, largest, largest])
+        x[4, 1], x[5, 1] = -up * 2.0 ** top, up * 0.96 * 2.0 ** top
+        x = x.to(dtype)
+        back = {t: native.ckpt_unpack(native.ckpt_pack(x.to(dev), fmt), t).cpu().to(F64) for t in (torch.float32, torch.bfloat16, torch.float16)}
+        inf = float("inf")
+        for t in (torch.float32, torch.bfloat16):
+            value = 2.0 ** top if top < 128 else inf
+            assert back[t][0, 0] == value and back[t][1, 0] == -value and back[t][4, 1] == -value
+        if top == 16:
+            got = back[torch.float16]
+            assert got[0, 0] == inf and got[1, 0] == -inf and got[4, 1] == -inf
+        finite = back[dtype]
+        for r, c in ((2, 0), (3, 0), (5, 1)):
+            assert abs(float(finite[r, c] - x[r, c].to(F64))) <= step / 2 * 2.0 ** top, (dtype, r)
+        assert bool((finite[:, 2:] == 0).all())                       # zeros beside them stay zeros: no NaN
