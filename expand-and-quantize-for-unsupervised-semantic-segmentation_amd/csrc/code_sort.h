@@ -12,9 +12,12 @@
 //   join       the partial sums of a run in the order of the tiles, and zeros for codes without rows
 //
 // For few rows all of it is one kernel (small): a workgroup owns a few codes, picks their rows out of all indices by itself, in
-// order, and sums them.  Measured (us, gradient of a lookup, small against sorted): 1000 rows, 8 x 256 x 128: 12 / 23; 2048 rows:
-// 16 / 25, and 40 / 26 where every row has the same code; 4096 rows: 22 / 22 (92 / 29 with one code); 4096 rows, 16384 x 16,
-// whose sort takes two passes: 12 / 38.  Hence up to 2048 rows, and up to 4096 where the sort would take more than one pass.
+// order, and sums them.  Measured (us a call, small against sorted; codes used evenly, by the square of a uniform number, all rows of
+// one code), gradient of a lookup, 8 x 256 x 128: 1024 rows 8.9 / 18, 13 / 18, 32 / 20; 2048 rows 9.8 / 19, 16 / 19, 54 / 21; 4096
+// rows, even and one code: 22 / 22, 92 / 29; quantiser's backward: 1024 rows 13 / 23, 19 / 23, 107 / 23; 2048 rows 13 / 23, 28 / 23,
+// 207 / 25.  4096 rows, 16384 x 16, whose sort takes two passes: 12 / 38.  Hence up to 2048 rows, and up to 4096 where the sort
+// would take more than one pass.  What it costs at worst goes by the rows of the busiest workgroup, not by the codes: 4096 rows on
+// 150000 x 32, even use, 300 neighbouring codes, one code: 17, 37, 37; on 5 million x 8: 51, 105, 90.
 //
 // An index outside [0, K) counts as the code K, which sorts last and has no sum.
 #pragma once
@@ -233,24 +236,98 @@ __global__ __launch_bounds__(64 * WAVES) void code_join_kernel(const WalkArgs w)
     }
 }
 
+// list[0 .. count) of 256 threads, in the order of its codes k0 .. k0 + 2^bits - 1; entries of one code stay in theirs.  Stable counting
+// passes of up to 8 bits: a wave has a quarter of the list, E entries a lane in registers, lanes of equal digit find each other by
+// one ballot a bit, and what the waves have of a digit lies in the order of the waves.  (A bitonic sort in LDS took 30 us for 4096
+// entries, this one 3 a pass.)  scratch: 4 KB, wave_sum: 4 numbers.
+template <int E>
+__device__ __forceinline__ void sort_list(CodePair* list, int count, uint32_t k0, int bits, f32x4* scratch, int* wave_sum) {
+    uint32_t* at = reinterpret_cast<uint32_t*>(scratch);   // (4 waves, 256 digits)
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint32_t* mine = at + wave * 256;
+    const int rounds = (count + 255) / 256, i0 = wave * rounds * 64 + lane;
+    for (int shift = 0; shift < bits; shift += 8) {
+        const int width = bits - shift < 8 ? bits - shift : 8;
+        __syncthreads();                                   // (behind the list's and the scratch's last use)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) at[w * 256 + tid] = 0;
+        __syncthreads();
+        CodePair held[E];
+        uint32_t rank[E];
+#pragma unroll
+        for (int r = 0; r < E; ++r) {
+            rank[r] = 0;
+            if (r < rounds) {                              // (uniform)
+                const bool in = i0 + r * 64 < count;
+                held[r] = list[in ? i0 + r * 64 : 0];
+                const uint32_t digit = ((held[r].code - k0) >> shift) & 255u;
+                uint64_t same = __ballot(in);
+                for (int b = 0; b < width; ++b) {
+                    const uint64_t set = __ballot((digit >> b) & 1);
+                    same &= (digit >> b) & 1 ? set : ~set;
+                }
+                if (in) {
+                    const uint32_t below = __popcll(same & ((1ull << lane) - 1));
+                    // (all lanes read before the first of them writes: LDS operations of a wave stay in order)
+                    const uint32_t before = __hip_atomic_load(&mine[digit], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+                    if (below == 0) __hip_atomic_store(&mine[digit], before + (uint32_t)__popcll(same), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+                    rank[r] = before + below;
+                }
+            }
+        }
+        __syncthreads();
+        // a thread a digit: where its entries start, for each wave
+        uint32_t n[4], total = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            n[w] = at[w * 256 + tid];
+            total += n[w];
+        }
+        uint32_t scan = total;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t up = (uint32_t)__shfl_up((int)scan, o, 64);
+            if (lane >= o) scan += up;
+        }
+        if (lane == 63) wave_sum[wave] = (int)scan;
+        __syncthreads();
+        uint32_t start = scan - total;
+        for (int w = 0; w < wave; ++w) start += (uint32_t)wave_sum[w];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            at[w * 256 + tid] = start;
+            start += n[w];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < E; ++r) {
+            if (r < rounds && i0 + r * 64 < count) list[mine[((held[r].code - k0) >> shift) & 255u] + rank[r]] = held[r];
+        }
+    }
+    __syncthreads();
+}
+
 // All in one for few rows: the workgroup's codes are [k0, k0 + codes).  Its rows come out of the indices in row order, eight
-// indices a thread at a time, and are put in the order of their codes by a bitonic sort of (code, row) where they are few
-// (256, a thread each); groups of lanes then walk the codes, several to a code where there are more groups than codes.  Where
-// one code has most of the rows, everybody walks the unsorted list once for each code.  The last workgroup has the rows without a
-// code too, for their own outputs.
-template <class Op, int LPR, int CAP>                     // CAP: most rows
+// indices a thread at a time, and are put in the order of their codes: by a bitonic sort of (code, row) in registers where they
+// are few (256, a thread each), by sort_list where they are more.  Groups of lanes then walk the codes, several to a code where
+// there are more groups than codes; runs of more than kRun rows are walked by all the groups together, one run after the other.
+// Of up to kFew codes with many rows, everybody walks the unsorted list once for each code, which is cheaper than the sort (2048
+// rows, 8 x 256 x 128, two codes a workgroup, 40 % of the rows on one code, gradient of a lookup: 27 us, 30 sorted) and dearer with
+// more codes (4096 rows, 150000 x 32, 147 codes a workgroup, 300 neighbouring codes in use: 700 us, 39 sorted).  The last workgroup
+// has the rows without a code too, where rows have an output of their own.
+template <class Op, int LPR, int CAP>                     // CAP: most rows, a power of two
 __global__ __launch_bounds__(256) void code_small_kernel(const Op op, const IndexView index, float* __restrict__ out_all, int rows,
                                                         uint32_t K, int d, int codes) {
-    constexpr int SLOTS = 256 / LPR, PER = 8, FLIGHT = Op::kOwn ? 4 : 8;
+    constexpr int SLOTS = 256 / LPR, PER = 8, FLIGHT = Op::kOwn ? 4 : 8, kRun = 64, kFew = 4;
     __shared__ CodePair list[CAP];
     __shared__ f32x4 share[256];
-    __shared__ int wave_count[PER][4];
+    __shared__ int wave_count[PER][4], runs, run_at[CAP / kRun];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, slot = tid / LPR;
     const int p = blockIdx.y, col = (int)blockIdx.z * 256 + (tid % LPR) * 4;
     const bool live = col < d, whole = (d & 3) == 0;
     const uint32_t k0 = blockIdx.x * (uint32_t)codes;
     const uint32_t kend = k0 + codes < K ? k0 + codes : K;
-    const uint32_t k1 = blockIdx.x == gridDim.x - 1 ? K + 1 : kend;
+    const uint32_t k1 = Op::kOwn && blockIdx.x == gridDim.x - 1 ? K + 1 : kend;
     int count = 0;
     for (int r0 = 0; r0 < rows; r0 += 256 * PER) {
         uint32_t k[PER];
@@ -277,17 +354,18 @@ __global__ __launch_bounds__(256) void code_small_kernel(const Op op, const Inde
     }
     float* out = out_all + (int64_t)p * K * d + col;
     const bool sums = out_all != nullptr;
-    auto sum_range = [&](int lo, int hi) {
+    auto sum_range = [&](auto flight, int lo, int hi) {
+        constexpr int F = decltype(flight)::value;         // rows in flight
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-        for (int j = lo; j < hi; j += 4) {
-            typename Op::Row row[4];
-            f32x4 v[4];
+        for (int j = lo; j < hi; j += F) {
+            typename Op::Row row[F];
+            f32x4 v[F];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) row[i] = op.template load<false>(list[j + i < hi ? j + i : hi - 1], p, live ? col : 0);
+            for (int i = 0; i < F; ++i) row[i] = op.template load<false>(list[j + i < hi ? j + i : hi - 1], p, live ? col : 0);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = op.value(row[i]);
+            for (int i = 0; i < F; ++i) v[i] = op.value(row[i]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < F; ++i)
                 if (j + i < hi) {
                     acc += v[i];
                     op.template own<false>(row[i], list[j + i].row, p, col);
@@ -295,9 +373,62 @@ __global__ __launch_bounds__(256) void code_small_kernel(const Op op, const Inde
         }
         return acc;
     };
-    if (count <= 256) {
-        // codes of this workgroup fit 16 bits beside the row's 11 only where they are few; 64-bit keys always do
-        uint64_t key = tid < count ? (uint64_t)list[tid].code << 32 | list[tid].row : ~0ull;
+    // the sum of every group's share of a code's rows, written (called by the whole workgroup)
+    auto store_joined = [&](uint32_t k, f32x4 acc) {
+#pragma unroll
+        for (int o = 32; o >= LPR; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], o, 64);
+        if (lane < LPR) share[wave * LPR + lane] = acc;
+        __syncthreads();
+        if (tid < LPR && live) {
+            for (int w = 1; w < 4; ++w) acc += share[w * LPR + tid];
+            store_cols(out + (int64_t)k * d, acc, col, d, whole);
+        }
+        __syncthreads();
+    };
+    const int n = (int)(k1 - k0);
+    if (__builtin_expect(count > 256 && n <= kFew, 0)) {
+        const int lo = count * slot / SLOTS, hi = count * (slot + 1) / SLOTS;
+        for (uint32_t k = k0; k < k1; ++k) {
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+            for (int j = lo; j < hi; j += FLIGHT) {
+                CodePair pr[FLIGHT];
+                bool any = false;
+#pragma unroll
+                for (int i = 0; i < FLIGHT; ++i) {
+                    pr[i] = list[j + i < hi ? j + i : hi - 1];
+                    any |= pr[i].code == k;
+                }
+                if (!any) continue;
+                typename Op::Row row[FLIGHT];
+#pragma unroll
+                for (int i = 0; i < FLIGHT; ++i) row[i] = op.template load<false>(pr[i], p, live ? col : 0);
+#pragma unroll
+                for (int i = 0; i < FLIGHT; ++i) {
+                    const f32x4 v = op.value(row[i]);
+                    if (j + i < hi && pr[i].code == k) {
+                        acc += v;
+                        op.template own<false>(row[i], pr[i].row, p, col);
+                    }
+                }
+            }
+            if (sums && k < kend) store_joined(k, acc);    // (uniform)
+        }
+        return;
+    }
+    auto key_of = [](const CodePair& at) { return (uint64_t)at.code << 32 | at.row; };
+    auto first_of = [&](uint32_t k) {                      // the first entry whose code is not below k
+        int lo = 0, hi = count;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (list[mid].code < k) lo = mid + 1;
+            else hi = mid;
+        }
+        return lo;
+    };
+    if (__builtin_expect(count <= 256, 1)) {
+        uint64_t key = tid < count ? key_of(list[tid]) : ~0ull;
         for (int width = 2; width <= 256; width *= 2) {
             if (width / 2 >= count) break;                 // (uniform: everything behind `count` is the largest key already)
             for (int step = width / 2; step > 0; step /= 2) {
@@ -316,69 +447,47 @@ __global__ __launch_bounds__(256) void code_small_kernel(const Op op, const Inde
         }
         if (tid < count) list[tid] = CodePair{(uint32_t)(key >> 32), (uint32_t)key};
         __syncthreads();
-        auto first_of = [&](uint32_t k) {                  // the first entry whose code is not below k
-            int lo = 0, hi = count;
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (list[mid].code < k) lo = mid + 1;
-                else hi = mid;
-            }
-            return lo;
-        };
-        const int n = (int)(k1 - k0);
-        const int parts = n < SLOTS ? SLOTS / n : 1;       // groups that share a code
-        for (int c0 = 0; c0 < n; c0 += SLOTS / parts) {
-            const int c = c0 + slot / parts, part = slot % parts;
-            const bool mine = slot / parts < SLOTS / parts && c < n;
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-            if (mine) {
-                const int lo = first_of(k0 + c), hi = first_of(k0 + c + 1), len = hi - lo;
-                if (Op::kOwn || k0 + c < kend) acc = sum_range(lo + len * part / parts, lo + len * (part + 1) / parts);
-            }
-            if (!sums) continue;
-            if (parts > 1) {                               // (then there is one round)
-                share[tid] = acc;
-                __syncthreads();
-                if (mine && part == 0)
-                    for (int j = 1; j < parts; ++j) acc += share[tid + j * LPR];
-            }
-            if (mine && part == 0 && live && k0 + c < kend) store_cols(out + (int64_t)(k0 + c) * d, acc, col, d, whole);
-        }
-        return;
+    } else {
+        bool other = false;
+        for (int j = tid; j < count; j += 256) other |= list[j].code != list[0].code;
+        if (__syncthreads_or(other)) sort_list<CAP / 256>(list, count, k0, 32 - __clz(n - 1), share, wave_count[0]);
     }
-    // (several rows in flight where any of their entries has the code: one codeword may own all the rows)
-    const int lo = (int)((int64_t)count * slot / SLOTS), hi = (int)((int64_t)count * (slot + 1) / SLOTS);
-    for (uint32_t k = k0; k < (Op::kOwn ? k1 : kend); ++k) {
+    // the long runs of a workgroup that may have some
+    const bool many = n > kFew && count > kRun;
+    if (__builtin_expect(many, 0)) {
+        if (tid == 0) runs = 0;
+        __syncthreads();
+        for (int j = tid; j + kRun < count; j += 256)      // (in any order: every run has a sum of its own)
+            if (list[j + kRun].code == list[j].code && (j == 0 || list[j - 1].code != list[j].code)) run_at[atomicAdd(&runs, 1)] = j;
+        __syncthreads();
+    }
+    const int parts = n < SLOTS ? SLOTS / n : 1;           // groups that share a code
+    for (int c0 = 0; c0 < n; c0 += SLOTS / parts) {
+        const int c = c0 + slot / parts, part = slot % parts;
+        bool mine = slot / parts < SLOTS / parts && c < n;
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-        for (int j = lo; j < hi; j += FLIGHT) {
-            CodePair pr[FLIGHT];
-            bool any = false;
-#pragma unroll
-            for (int i = 0; i < FLIGHT; ++i) {
-                pr[i] = list[j + i < hi ? j + i : hi - 1];
-                any |= pr[i].code == k;
-            }
-            if (!any) continue;
-            typename Op::Row row[FLIGHT];
-#pragma unroll
-            for (int i = 0; i < FLIGHT; ++i) row[i] = op.template load<false>(pr[i], p, live ? col : 0);
-#pragma unroll
-            for (int i = 0; i < FLIGHT; ++i) {
-                const f32x4 v = op.value(row[i]);
-                if (j + i < hi && pr[i].code == k) {
-                    acc += v;
-                    op.template own<false>(row[i], pr[i].row, p, col);
-                }
-            }
+        if (mine) {
+            const int lo = first_of(k0 + c), len = first_of(k0 + c + 1) - lo;
+            mine = !many || len <= kRun;
+            if (mine) acc = sum_range(std::integral_constant<int, 4>(), lo + len * part / parts, lo + len * (part + 1) / parts);
         }
-        if (!sums || k >= kend) continue;                  // (uniform)
-        share[tid] = acc;
-        __syncthreads();
-        if (slot == 0 && live) {
-            for (int j = 1; j < SLOTS; ++j) acc += share[j * LPR + tid];
-            store_cols(out + (int64_t)k * d, acc, col, d, whole);
+        if (!sums) continue;
+        if (parts > 1) {                                   // (then there is one round)
+            share[tid] = acc;
+            __syncthreads();
+            if (mine && part == 0)
+                for (int j = 1; j < parts; ++j) acc += share[tid + j * LPR];
         }
-        __syncthreads();
+        if (mine && part == 0 && live && k0 + c < kend) store_cols(out + (int64_t)(k0 + c) * d, acc, col, d, whole);
+    }
+    if (__builtin_expect(!many, 1)) return;
+    __syncthreads();                                       // (behind the readers of share)
+    for (int i = 0; i < runs; ++i) {
+        const int lo = run_at[i];
+        const uint32_t k = list[lo].code;
+        const int len = first_of(k + 1) - lo;
+        const f32x4 acc = sum_range(std::integral_constant<int, FLIGHT>(), lo + len * slot / SLOTS, lo + len * (slot + 1) / SLOTS);
+        if (sums && k < kend) store_joined(k, acc);        // (uniform)
     }
 }
 

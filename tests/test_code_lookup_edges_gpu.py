@@ -58,3 +58,64 @@ def test_vector_quantizer_carries_tangents(pkg, dev):
         vq.codebook.weight = fwd.make_dual(weight.requires_grad_(True), t)
         tangent = fwd.unpack_dual(vq(z)[1]["loss"]).tangent
     assert abs(float((grad.to(F64) * t.to(F64)).sum() - tangent.detach().to(F64))) <= 1600 * U * float((grad.abs().to(F64) * t.abs().to(F64)).sum())
+
+
+def clustered(kind, num_pq, rows, k, seed):
+    g = torch.Generator().manual_seed(seed)
+    near = torch.randint(0, k, (num_pq, rows), generator=g)
+    if kind == "low":                                       # a vocabulary in the order of its frequency
+        near = (torch.rand(num_pq, rows, generator=g, dtype=F64) ** 6 * k).long().clamp_(max=k - 1)
+    elif kind == "cluster":
+        near = torch.randint(0, min(k, 300), (num_pq, rows), generator=g)
+    elif kind == "busy":                                    # a tenth of the rows on the last code, a tenth on its neighbour
+        u = torch.rand(num_pq, rows, generator=g)
+        near = torch.where(u < 0.1, torch.full_like(near, k - 1), torch.where(u < 0.2, torch.full_like(near, max(k - 2, 0)), near))
+    elif kind == "padding":
+        near = torch.where(torch.rand(num_pq, rows, generator=g) < 0.4, torch.full_like(near, -1), near)
+    elif kind == "pairs":                                   # runs on either side of the border between one group's and all groups'
+        near = (torch.arange(rows) // 64 + torch.arange(rows) // 129).clamp_(max=k - 1).repeat(num_pq, 1)
+    return near
+
+
+@pytest.mark.parametrize("rows,num_pq,k,d", [(257, 1, 5000, 4), (2048, 1, 40000, 3), (2048, 2, 2000, 8), (4096, 1, 150000, 32), (4095, 2, 16384, 16),
+                                             (4096, 1, 2000000, 2), (3000, 1, 70000, 128), (2000, 1, 3000, 700), (1999, 3, 900, 60), (600, 1, 1, 24)])
+def test_lookup_gradient_of_few_rows_on_neighbouring_codes(rows, num_pq, k, d, native, dev):
+    """More than 256 rows on the codes of one workgroup, in every mixture of long and short runs.  Whole numbers add exactly."""
+    g = torch.randint(-8, 9, (rows, num_pq * d), generator=torch.Generator().manual_seed(rows)).float()
+    for kind in ("low", "cluster", "busy", "padding", "pairs"):
+        idx = clustered(kind, num_pq, rows, k, 31)
+        want = torch.zeros(num_pq, k, d)
+        for p in range(num_pq):
+            ok = idx[p] >= 0
+            want[p].index_add_(0, idx[p][ok], g.reshape(rows, num_pq, d)[ok, p])
+        got = native.code_lookup_grad(g.to(dev), idx.to(dev), k)
+        assert torch.equal(got.cpu(), want), kind
+        x = torch.randn(rows, num_pq * d, device=dev)
+        assert torch.equal(native.code_lookup_grad(x, idx.to(dev), k), native.code_lookup_grad(x, idx.to(dev), k)), kind
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("rows,num_pq,k,d", [(4096, 1, 5000, 16), (2048, 2, 2000, 32), (1500, 1, 1800, 128), (1000, 4, 700, 64)])
+def test_quantiser_backward_of_few_rows_on_neighbouring_codes(rows, num_pq, k, d, fmt, native, dev):
+    """The same for the quantiser's backward, whose rows have gradients of their own, those of no codeword among them: each row's
+    is what the call gives for these rows without the clustering (its own to the bit), the codebooks' agree with fp64 sums."""
+    for kind in ("low", "cluster", "busy", "padding", "pairs"):
+        idx = clustered(kind, num_pq, rows, k, 32)
+        g = torch.Generator().manual_seed(33)
+        z, g_zq = torch.randn(rows, num_pq * d, generator=g), torch.randn(rows, num_pq * d, generator=g) * 1e-3
+        books = torch.randn(num_pq, k, d, generator=g) * d ** -0.5
+        kept, gv = native.ckpt_pack(z.to(dev), fmt), torch.tensor(0.7, device=dev)
+        gz, gb = native.pq_st_backward_ckpt(kept, books.to(dev), idx.to(dev), g_zq.to(dev), gv, 0.25, 1.5)
+        # rows one by one through codebooks of their own: codeword r is row r's
+        own = torch.stack([torch.where((idx[p] >= 0).unsqueeze(1), books[p][idx[p].clamp(min=0)], torch.zeros(1, d)) for p in range(num_pq)])
+        each = torch.arange(rows).repeat(num_pq, 1)
+        apart, _ = native.pq_st_backward_ckpt(kept, own.to(dev), each.to(dev), g_zq.to(dev), gv, 0.25, 1.5)
+        assert torch.equal(gz, apart), kind
+        z3 = native.ckpt_unpack(kept).cpu().to(F64).reshape(rows, num_pq, d)
+        zn, s = z3 / z3.norm(dim=-1, keepdim=True), 0.7 * 2.0 / (rows * num_pq * d) * 1.5
+        for p in range(num_pq):
+            ok, i = idx[p] >= 0, idx[p].clamp(min=0)
+            want, size, count = torch.zeros(k, d, dtype=F64), torch.zeros(k, d, dtype=F64), torch.bincount(i[ok], minlength=k).to(F64).unsqueeze(1)
+            want.index_add_(0, i[ok], s * (books[p][i[ok]].to(F64) - zn[ok, p]))
+            size.index_add_(0, i[ok], s * (books[p][i[ok]].to(F64).abs() + zn[ok, p].abs()))
+            assert bool(((gb[p].cpu().to(F64) - want).abs() <= (count + 16) * U * size).all()), kind   # 16 u a term, u an addition
