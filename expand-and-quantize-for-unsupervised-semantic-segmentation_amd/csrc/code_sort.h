@@ -175,7 +175,8 @@ __global__ __launch_bounds__(256) void code_accumulate_kernel(const Op op, const
 
 // WAVES = 4: a wave owns a code, and the chain of partial sums of a long run is shared by the workgroup's four waves.  WAVES = 16,
 // where there are few codes, i.e. long runs: a workgroup owns a code (102045 rows, 5 x 2 x 32, gradient of a lookup: 42 us, 65 us
-// with four waves; 102400 rows, 8 x 256 x 128: 100 / 96 us, hence at most 1024 codes).
+// with four waves; 102400 rows, 8 x 256 x 128: 100 / 96 us; hence at most 1024 workgroups, a codeword of more than 256 columns
+// taking several: 3000 rows, 1000 x 4096: 81 us with 16000 of them, 36 with four waves each).
 template <int LPR, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void code_join_kernel(const WalkArgs w) {
     constexpr int SLOTS = 64 / LPR, CODES = WAVES == 4 ? 4 : 1, kLong = 16 * SLOTS, F = 8;
@@ -520,7 +521,7 @@ int walk_launch_lpr(const Op& op, const SortPlan& s, const IndexView& index, cha
     else hipLaunchKernelGGL((code_accumulate_kernel<Op, LPR, 2>), grid, dim3(256), 0, stream, op, w);
     rc = check_launch("code_accumulate_kernel");
     if (rc != EQUSS_OK || !out) return rc;
-    if ((int64_t)s.K * s.num_pq <= 1024) hipLaunchKernelGGL((code_join_kernel<LPR, 16>), dim3(s.K, s.num_pq, cchunks), dim3(1024), 0, stream, w);
+    if ((int64_t)s.K * s.num_pq * cchunks <= 1024) hipLaunchKernelGGL((code_join_kernel<LPR, 16>), dim3(s.K, s.num_pq, cchunks), dim3(1024), 0, stream, w);
     else hipLaunchKernelGGL((code_join_kernel<LPR, 4>), dim3((s.K + 3) / 4, s.num_pq, cchunks), dim3(256), 0, stream, w);
     return check_launch("code_join_kernel");
 }
