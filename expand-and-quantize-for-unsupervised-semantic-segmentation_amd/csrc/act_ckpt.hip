@@ -251,7 +251,7 @@ bool walk(Walk& w, int64_t rows, int width, int type, int64_t& grid) {
     const int64_t spread = (rows + 1023) / 1024;   // few rows: as many workgroups as rows
     if (r > spread) r = spread;
     if (r < 1) r = 1;
-    while ((rows + r - 1) / r > 0x7fffffff) r *= 2;
+    while ((rows + r - 1) / r > equss::max_blocks(kThreads)) r *= 2;
     w.rows_wg = (int)r;
     w.magic = r == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + w.units_row - 1) / w.units_row);
     grid = (rows + r - 1) / r;

@@ -207,6 +207,8 @@ extern "C" int equss_code_lookup(const void* idx, int index_type, int64_t stride
     a.magic_code = magic(a.units_code);
     if (whole && (int64_t)a.units_row * a.units_code >= ((int64_t)1 << 32))
         return equss::fail(EQUSS_E_UNSUPPORTED, "equss_code_lookup: num_pq=%d d=%d", num_pq, d);
+    if ((rows + r - 1) / r > equss::max_blocks(256))
+        return equss::fail(EQUSS_E_UNSUPPORTED, "equss_code_lookup: %lld rows of %d elements", (long long)rows, a.width);
     const dim3 grid((unsigned)((rows + r - 1) / r));
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
 #define EQUSS_LOOKUP(T)                                                                                 \

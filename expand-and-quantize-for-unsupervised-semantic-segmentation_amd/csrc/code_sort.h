@@ -98,6 +98,7 @@ struct WalkArgs {
     float* partial;                     // (num_pq, tiles, 2, dpad): a tile's head and tail
     float* out;                         // (num_pq, K, d), or null: only the rows' own outputs are wanted
     int64_t rows, tiles;
+    int64_t code0;                      // the join's first code
     int tile, d, dpad;
     uint32_t K;
 };
@@ -208,7 +209,7 @@ __global__ __launch_bounds__(64 * WAVES) void code_join_kernel(const WalkArgs w)
             for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], o, 64);
         return acc;
     };
-    const int64_t k0 = (int64_t)blockIdx.x * CODES;
+    const int64_t k0 = w.code0 + (int64_t)blockIdx.x * CODES;
     int64_t at[CODES + 1];
 #pragma unroll
     for (int c = 0; c <= CODES; ++c) at[c] = starts[k0 + c <= (int64_t)w.K ? k0 + c : (int64_t)w.K];
@@ -514,7 +515,7 @@ int walk_launch_lpr(const Op& op, const SortPlan& s, const IndexView& index, cha
     w.pairs = reinterpret_cast<const CodePair*>(ws + at);
     w.starts = reinterpret_cast<const uint32_t*>(ws + s.starts);
     w.partial = reinterpret_cast<float*>(ws + s.partial);
-    w.out = out; w.rows = s.rows; w.tiles = s.tiles; w.tile = s.tile; w.d = d; w.dpad = (d + 3) / 4 * 4; w.K = s.K;
+    w.out = out; w.rows = s.rows; w.code0 = 0; w.tiles = s.tiles; w.tile = s.tile; w.d = d; w.dpad = (d + 3) / 4 * 4; w.K = s.K;
     constexpr int TILES_WG = 4 * (64 / LPR);
     const dim3 grid((unsigned)((s.tiles + TILES_WG - 1) / TILES_WG), s.num_pq, cchunks);
     if (s.tile == kTile) hipLaunchKernelGGL((code_accumulate_kernel<Op, LPR, 1>), grid, dim3(256), 0, stream, op, w);
@@ -522,7 +523,11 @@ int walk_launch_lpr(const Op& op, const SortPlan& s, const IndexView& index, cha
     rc = check_launch("code_accumulate_kernel");
     if (rc != EQUSS_OK || !out) return rc;
     if ((int64_t)s.K * s.num_pq * cchunks <= 1024) hipLaunchKernelGGL((code_join_kernel<LPR, 16>), dim3(s.K, s.num_pq, cchunks), dim3(1024), 0, stream, w);
-    else hipLaunchKernelGGL((code_join_kernel<LPR, 4>), dim3((s.K + 3) / 4, s.num_pq, cchunks), dim3(256), 0, stream, w);
+    else
+        for (constexpr int64_t kMost = max_blocks(256) * 4; w.code0 < (int64_t)s.K; w.code0 += kMost) {   // (one launch below 67 million codes)
+            const int64_t left = (int64_t)s.K - w.code0, codes = left < kMost ? left : kMost;
+            hipLaunchKernelGGL((code_join_kernel<LPR, 4>), dim3((unsigned)((codes + 3) / 4), s.num_pq, cchunks), dim3(256), 0, stream, w);
+        }
     return check_launch("code_join_kernel");
 }
 

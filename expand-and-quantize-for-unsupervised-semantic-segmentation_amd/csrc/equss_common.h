@@ -62,6 +62,9 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2_t));
 }
 
+// Workgroups of a launch with `threads` each: HIP takes fewer than 2^32 threads in a dimension.
+constexpr int64_t max_blocks(int threads) { return (((int64_t)1 << 32) - 1) / threads; }
+
 // The bits of one 32-bit value as another type, by value: __builtin_bit_cast applied to a vector's element (v[i], which is an
 // lvalue) takes the vector's first element whatever i is.
 template <class To>

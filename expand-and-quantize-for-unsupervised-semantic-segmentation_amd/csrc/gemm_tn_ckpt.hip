@@ -562,6 +562,8 @@ int tile_of(int64_t rows, int M, int N, bool mask) {
     return !mask && (double)rows * M * N >= 2e10 && small > 3 * large ? 256 : 128;
 }
 
+constexpr int kMostCols = 1 << 30;     // columns are 32-bit numbers, and rounded up
+
 // partial products and, behind them, partial bias sums; nothing where one row range writes the results
 size_t workspace(const Plan& p, int M, int N) {
     return p.splits == 1 ? 0 : ((size_t)p.splits * M * N + (size_t)p.bias_splits * M) * sizeof(float);
@@ -570,7 +572,7 @@ size_t workspace(const Plan& p, int M, int N) {
 }  // namespace
 
 extern "C" size_t equss_gemm_tn_ckpt_workspace_bytes(int64_t rows, int M, int N) {
-    if (rows < 0 || M <= 0 || N <= 0) return 0;
+    if (rows < 0 || M <= 0 || N <= 0 || M > kMostCols || N > kMostCols) return 0;
     // with a mask or without, and the narrow kernel, which stands in where leading dimensions are too long for the others
     const int tiles[3] = {tile_of(rows, M, N, false), tile_of(rows, M, N, true), 0};
     size_t most = 0;
@@ -585,6 +587,7 @@ extern "C" int equss_gemm_tn_ckpt(const void* a, int64_t lda, const void* codes,
                                   int fmt, const void* relu_codes, int64_t ld_relu, float* C, int64_t ldc, float* bias, int64_t rows,
                                   int M, int N, void* workspace_ptr, size_t workspace_bytes, void* stream) {
     if (rows < 0 || M <= 0 || N <= 0) return equss::fail(EQUSS_E_SHAPE, "equss_gemm_tn_ckpt: rows=%lld M=%d N=%d", (long long)rows, M, N);
+    if (M > kMostCols || N > kMostCols) return equss::fail(EQUSS_E_UNSUPPORTED, "equss_gemm_tn_ckpt: M=%d N=%d (at most %d)", M, N, kMostCols);
     if (fmt != EQUSS_CKPT_INT8 && fmt != EQUSS_CKPT_E4M3) return equss::fail(EQUSS_E_UNSUPPORTED, "equss_gemm_tn_ckpt: format %d", fmt);
     if (!C || (rows > 0 && (!a || !codes || !scales))) return equss::fail(EQUSS_E_NULL, "equss_gemm_tn_ckpt: null pointer argument");
     Args g;
@@ -604,7 +607,7 @@ extern "C" int equss_gemm_tn_ckpt(const void* a, int64_t lda, const void* codes,
     if (need > 0 && (!workspace_ptr || workspace_bytes < need || ((uintptr_t)workspace_ptr % 16) != 0))
         return equss::fail(EQUSS_E_WORKSPACE, "equss_gemm_tn_ckpt: workspace of %zu bytes, 16-byte aligned, needed", need);
     const int64_t blocks = (int64_t)p.tiles_m * p.tiles_n * p.splits;
-    if (blocks > 0x7fffffff || (p.rows_split + BK - 1) / BK > 0x7fffffff)
+    if (blocks + 7 > equss::max_blocks(2 * 256) || (p.rows_split + BK - 1) / BK > 0x7fffffff)
         return equss::fail(EQUSS_E_UNSUPPORTED, "equss_gemm_tn_ckpt: %lld rows, M=%d N=%d", (long long)rows, M, N);
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     g.a = reinterpret_cast<const u16*>(a); g.lda = lda;

@@ -441,7 +441,7 @@ int equss_ckpt_unpack(const void* codes, int64_t ld_codes, const void* scales, i
  *   relu_codes (rows, M) codes of a checkpoint of either format, or NULL: a[r][m] counts only where the code is > 0, in both sums
  *   C      (M, N) fp32 out, leading dimension ldc; bias (M) fp32 out or NULL
  *   workspace equss_gemm_tn_ckpt_workspace_bytes() bytes, 16-byte aligned (may be NULL where that is 0)
- * M, N and rows are any size (rows == 0 gives zeros).  bf16 MFMA on exactly the kept values, fp32 accumulation; the partial sums
+ * M and N up to 2^30, rows any number (0 gives zeros).  bf16 MFMA on exactly the kept values, fp32 accumulation; the partial sums
  * of the row ranges are added in a fixed order: equal calls give equal bits. */
 size_t equss_gemm_tn_ckpt_workspace_bytes(int64_t rows, int M, int N);
 int equss_gemm_tn_ckpt(const void* a, int64_t lda, const void* codes, int64_t ld_codes, const void* scales, int64_t ld_scales,
@@ -465,7 +465,8 @@ int equss_pq_st_backward_ckpt(const void* codes, int64_t ld_codes, const void* s
  * (-1 marks a place without a token).
  *   idx   (num_pq, rows) of index_type EQUSS_I64 / _I32 / _I16, element (p, r) at idx[p*stride_p + r*stride_r]
  *   books (num_pq, K, d) of type EQUSS_F32 / _BF16 / _F16, 16-byte aligned; out (rows, num_pq*d) of the same type, any alignment
- * The product is taken in fp32 and rounded once. */
+ * The product is taken in fp32 and rounded once.  num_pq <= 65535, num_pq * d <= 2^24, K < 2^31, rows < 2^31 - 256 (here and in
+ * the gradient). */
 int equss_code_lookup(const void* idx, int index_type, int64_t stride_p, int64_t stride_r, const void* books, int type,
                       float scale, void* out, int64_t ld_out, int64_t rows, int num_pq, int64_t K, int d, void* stream);
 
@@ -473,7 +474,7 @@ int equss_code_lookup(const void* idx, int index_type, int64_t stride_p, int64_t
  *   g (rows, num_pq*d) of type EQUSS_F32 / _BF16 / _F16, any alignment; g_books (num_pq, K, d) fp32 out, 16-byte aligned, written
  *   whole (codes without rows get zeros; indices outside [0, K) add to none)
  *   workspace equss_code_sums_sorted_workspace_bytes() bytes, 256-byte aligned (may be NULL where that is 0)
- * fp32 sums in a fixed order: equal calls give equal bits.  rows < 2^31 - 256. */
+ * fp32 sums in a fixed order: equal calls give equal bits. */
 size_t equss_code_sums_sorted_workspace_bytes(int64_t rows, int num_pq, int64_t K, int d);
 int equss_code_lookup_grad(const void* g, int type, int64_t ld_g, const void* idx, int index_type, int64_t stride_p,
                            int64_t stride_r, float scale, float* g_books, int64_t rows, int num_pq, int64_t K, int d,

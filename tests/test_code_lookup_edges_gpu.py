@@ -119,3 +119,16 @@ def test_quantiser_backward_of_few_rows_on_neighbouring_codes(rows, num_pq, k, d
             want.index_add_(0, i[ok], s * (books[p][i[ok]].to(F64) - zn[ok, p]))
             size.index_add_(0, i[ok], s * (books[p][i[ok]].to(F64).abs() + zn[ok, p].abs()))
             assert bool(((gb[p].cpu().to(F64) - want).abs() <= (count + 16) * U * size).all()), kind   # 16 u a term, u an addition
+
+
+def test_lookup_gradient_of_more_codes_than_one_launch_joins(native, dev):
+    """67 million codes and a few more: the codes behind the first launch's are written like the others, zeros included."""
+    rows, k, d = 4200, (1 << 26) + 5, 2
+    g = torch.randint(-8, 9, (rows, d), generator=torch.Generator().manual_seed(41)).float()
+    last = torch.tensor([0, 1, (1 << 26) - 5, (1 << 26) - 4, (1 << 26) - 3, 1 << 26, k - 2, k - 1, k, -1])
+    idx = last[torch.randint(0, len(last), (1, rows), generator=torch.Generator().manual_seed(42))]
+    got = native.code_lookup_grad(g.to(dev), idx.to(dev), k)
+    ok = (idx[0] >= 0) & (idx[0] < k)
+    want = torch.zeros(1, k, d, device=dev)
+    want[0].index_add_(0, idx[0][ok].to(dev), g[ok].to(dev))          # whole numbers: exact in any order
+    assert torch.equal(got, want) and int((got != 0).any(-1).sum()) >= 7
