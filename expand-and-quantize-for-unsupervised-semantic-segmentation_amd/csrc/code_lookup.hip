@@ -52,7 +52,7 @@ struct LookupArgs {
 
 __device__ __forceinline__ uint32_t divide(uint32_t a, uint32_t magic, uint32_t by_one) { return by_one ? a : __umulhi(a, magic); }
 
-// WHOLE: a code's d elements are whole 16-byte units and rows start on 16 bytes; otherwise a unit is gathered element by element
+// WHOLE: a code's d elements are whole 16-byte units (fewer than 65536 of them) and rows start on 16 bytes; otherwise a unit is gathered element by element
 // and stored at whatever address it has.
 template <int T, bool WHOLE>
 __global__ __launch_bounds__(256) void code_lookup_kernel(const LookupArgs a) {
@@ -193,20 +193,19 @@ extern "C" int equss_code_lookup(const void* idx, int index_type, int64_t stride
     a.width = num_pq * d;
     if (ld_out < a.width || ((uintptr_t)books % 16) != 0 || ((uintptr_t)out % es) != 0)
         return equss::fail(EQUSS_E_ALIGN, "equss_code_lookup: books 16-byte aligned, rows of %d elements", a.width);
-    const bool whole = (d % v) == 0 && (ld_out % v) == 0 && ((uintptr_t)out % 16) == 0;
     a.units_row = (a.width + v - 1) / v;
+    // (the division by units_code by multiplication: units_row * units_code below 2^32)
+    const bool whole = (d % v) == 0 && (ld_out % v) == 0 && ((uintptr_t)out % 16) == 0 && (int64_t)a.units_row * (d / v) < ((int64_t)1 << 32);
     a.units_code = whole ? d / v : 1;
     int64_t r = 2048 / a.units_row;
     const int64_t spread = (rows + 2047) / 2048;
     if (r > spread) r = spread;
     if (r < 1) r = 1;
-    // (the products below 2^32 that the divisions by multiplication need: r * units_row <= 2048 units, 2^24 / 4 units a row alone)
+    // (the division by units_row: r * units_row <= 2048 units, or a row alone)
     a.rows_wg = (int)r;
     auto magic = [](int n) { return n == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + n - 1) / n); };
     a.magic_row = magic(a.units_row);
     a.magic_code = magic(a.units_code);
-    if (whole && (int64_t)a.units_row * a.units_code >= ((int64_t)1 << 32))
-        return equss::fail(EQUSS_E_UNSUPPORTED, "equss_code_lookup: num_pq=%d d=%d", num_pq, d);
     if ((rows + r - 1) / r > equss::max_blocks(256))
         return equss::fail(EQUSS_E_UNSUPPORTED, "equss_code_lookup: %lld rows of %d elements", (long long)rows, a.width);
     const dim3 grid((unsigned)((rows + r - 1) / r));

@@ -132,3 +132,17 @@ def test_lookup_gradient_of_more_codes_than_one_launch_joins(native, dev):
     want = torch.zeros(1, k, d, device=dev)
     want[0].index_add_(0, idx[0][ok].to(dev), g[ok].to(dev))          # whole numbers: exact in any order
     assert torch.equal(got, want) and int((got != 0).any(-1).sum()) >= 7
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("num_pq,d", [(1, 1 << 18), (1, 1 << 20), (2, 1 << 19)])
+def test_lookup_of_the_widest_codewords(num_pq, d, dtype, native, dev):
+    """Codewords whose 16-byte units pass the range of the division by multiplication."""
+    books = torch.randn(num_pq, 3, d, generator=torch.Generator().manual_seed(43)).to(dtype)
+    idx = torch.tensor([[2, 0, -1, 1, 3]]).repeat(num_pq, 1)
+    got = native.code_lookup(idx.to(dev), books.to(dev), 0.5).cpu().reshape(5, num_pq, d)
+    for r, k in enumerate(idx[0].tolist()):
+        want = (books[:, k].float() * 0.5).to(dtype) if 0 <= k < 3 else torch.zeros(num_pq, d, dtype=dtype)
+        assert torch.equal(got[r], want), r
+    g = torch.ones(5, num_pq * d, dtype=dtype, device=dev)
+    assert torch.equal(native.code_lookup_grad(g, idx.to(dev), 3).cpu(), torch.ones(num_pq, 3, d))
