@@ -469,6 +469,10 @@ class Codebook(nn.Module):
     """One sub-quantiser (model/dino_pqgo.py:460-705): parameter ``embedding.weight`` (K, d) drawn
     U(-1/K, 1/K); ``vq_count`` is a plain attribute, not a buffer, as in the reference (:494)."""
 
+    # what the training pass keeps its input in for the backward: "none" (fp32), "int8" or "e4m3" (l2 normalisation only); of the
+    # class, for modules that were saved whole before they had it
+    activation_checkpoint = "none"
+
     def __init__(self, num_codebook_vectors: int, latent_dim: int, beta=0.25, book=1.0, normalize: str = "none",
                  use_restart: bool = False, use_split: bool = False, use_weighted_sum: bool = False,
                  use_gumbel: bool = False, need_initialized: str = "kmeans", pq_dropout: float = 0.0,
@@ -497,8 +501,6 @@ class Codebook(nn.Module):
         self.use_restart, self.use_split = use_restart, use_split
         self.need_initialized = need_initialized
         self.jsd_ts = jsd_ts
-        # what the training pass keeps its input in for the backward: "none" (fp32), "int8" or "e4m3" (l2 normalisation only)
-        self.activation_checkpoint = "none"
 
     @torch.no_grad()
     def prepare_restart(self, vq_current_count: torch.Tensor, z_flat: torch.Tensor) -> None:
@@ -574,6 +576,10 @@ class ProductQuantizerWrapper(nn.Module):
     """model/dino_pqgo.py:708-776: ``quantizers`` is a ModuleList of ``num_pq`` Codebooks over equal
     channel groups.  All sub-spaces are assigned by ONE kernel launch instead of a python loop."""
 
+    # what the training pass keeps its input in for the backward: "none" (fp32), "int8" or "e4m3" (l2 normalisation only); of the
+    # class, for modules that were saved whole before they had it
+    activation_checkpoint = "none"
+
     def __init__(self, num_pq: int, num_codebook: int, embed_dim: int, beta: float = 0.25, book: float = 1.0,
                  normalize: Optional[str] = None, decay: float = 0.99, eps: float = 1e-5, use_restart: bool = False,
                  use_split: bool = False, use_gumbel: bool = False, use_weighted_sum: bool = False,
@@ -591,8 +597,6 @@ class ProductQuantizerWrapper(nn.Module):
             for _ in range(self.num_pq)])
         self._books = None
         self._books_key = None
-        # what the training pass keeps its input in for the backward: "none" (fp32), "int8" or "e4m3" (l2 normalisation only)
-        self.activation_checkpoint = "none"
 
     def lookup(self, z_index: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
         """The features that indices stand for.  (num_pq, b, h, w) integer, as DIONPQGO.forward stacks them -> (b, D, h, w);
@@ -657,6 +661,8 @@ class ProductQuantizerWrapper(nn.Module):
 
 class DIONPQGO(nn.Module):
     """model/dino_pqgo.py:15-154."""
+
+    _activation_checkpoint = "none"      # (of the class, for models that were saved whole before they had it)
 
     def __init__(self, cfg: dict, cfg_loss: dict):
         super().__init__()

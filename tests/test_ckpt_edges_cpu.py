@@ -1,6 +1,8 @@
 """What the checkpoint and lookup calls decide on the host, at the ends of their sizes: no GPU needed."""
 import ctypes
 
+import torch
+
 
 def test_partial_sums_of_wide_codewords_go_by_all_their_columns(native):
     """8192 rows of 4096 columns fill the chip with tiles of 32: 256 tiles with two partial sums of 4096 floats each, beside 8
@@ -24,3 +26,18 @@ def test_sizes_past_a_launch_are_refused_before_it(native):
 
     assert grad(1 << 20, 1 << 20) == grad(8, (1 << 31) - 1) == grad((1 << 31) - 1, 8) == grad((1 << 30) + 1, 8) == UNSUPPORTED
     assert lib.equss_gemm_tn_ckpt_workspace_bytes(1 << 20, (1 << 31) - 1, 8) == lib.equss_gemm_tn_ckpt_workspace_bytes(1 << 20, 8, (1 << 31) - 1) == 0
+
+
+def test_modules_saved_whole_before_they_had_the_setting(pkg, tmp_path):
+    """A pickled module brings its own attributes and nothing else: the setting's default comes from the class."""
+    model = pkg.build_model(pkg.configs.pqgo_config())
+    block = model.model.vq_blocks[0]
+    for module in (model.model, block, *block.quantizers):
+        for name in ("activation_checkpoint", "_activation_checkpoint"):
+            module.__dict__.pop(name, None)
+    torch.save(model, tmp_path / "model.pt")
+    back = torch.load(tmp_path / "model.pt", weights_only=False)            # (this test's own file)
+    block = back.model.vq_blocks[0]
+    assert back.model.activation_checkpoint == block.activation_checkpoint == block.quantizers[0].activation_checkpoint == "none"
+    back.model.activation_checkpoint = "e4m3"
+    assert back.model.activation_checkpoint == block.activation_checkpoint == "e4m3"
