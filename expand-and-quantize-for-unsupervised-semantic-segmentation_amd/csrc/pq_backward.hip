@@ -3,7 +3,7 @@
 // (rows, D) tensors).  With zn = z / max(|z|, 1e-12) per sub-space, emb = books[idx] and
 //     vq = mean_p( book * mse(emb, zn.detach()) + beta * mse(zn, emb.detach()) ),   zq = zn + (emb - zn).detach()
 // the gradients are, with s = g_vq * 2 / (rows * d * num_pq):
-//     d zn   = g_zq + beta * s * (zn - emb)          d z = (d zn - zn <zn, d zn>) / |z|
+//     d zn   = g_zq + beta * s * (zn - emb)          d z = (d zn - zn <zn, d zn>) / |z|   (d zn / 1e-12 where |z| < 1e-12)
 //     d books[p][k] = -book * s * sum over the rows with idx[p] = k of (zn - emb)
 // One pass over the rows: z, emb and g_zq are read once, d z written once; the codebook gradient is accumulated with
 // float atomic adds of whole sub-vectors (consecutive addresses, the shape the memory-side adders take at full rate).
@@ -50,7 +50,7 @@ __global__ __launch_bounds__(256) void pq_st_backward_kernel(const PqBwdArgs a) 
         f32x4 gq = {0.f, 0.f, 0.f, 0.f};
         if (a.g_zq) gq = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(a.g_zq + r * a.ld_g + colc));
         const float n2 = equss::group_sum<LPR>(z.x * z.x + z.y * z.y + z.z * z.z + z.w * z.w);
-        const float norm = fmaxf(sqrtf(n2), 1e-12f);   // F.normalize's eps
+        const float len = sqrtf(n2), norm = fmaxf(len, 1e-12f);   // F.normalize's eps
         f32x4 zn, df, gn;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -79,7 +79,8 @@ __global__ __launch_bounds__(256) void pq_st_backward_kernel(const PqBwdArgs a) 
             }
         }
         if (a.g_z) {
-            const float proj = equss::group_sum<LPR>(zn.x * gn.x + zn.y * gn.y + zn.z * gn.z + zn.w * gn.w);
+            float proj = equss::group_sum<LPR>(zn.x * gn.x + zn.y * gn.y + zn.z * gn.z + zn.w * gn.w);
+            if (len < 1e-12f) proj = 0.f;              // (the norm is a constant there, and has no gradient)
             f32x4 o;
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[i] = (gn[i] - zn[i] * proj) / norm;

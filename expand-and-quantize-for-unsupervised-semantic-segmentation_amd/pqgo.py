@@ -353,7 +353,7 @@ class _PQStraightThrough(torch.autograd.Function):
             g_zn = diff.mul_(beta * scale)
             if g_zq is not None:
                 g_zn += g_zq.reshape(n, num_pq, d)
-            proj = (zn * g_zn).sum(dim=-1, keepdim=True)
+            proj = (zn * g_zn).sum(dim=-1, keepdim=True) * (norm > 1e-12)     # (a clamped norm has no gradient)
             g_rows = (g_zn.addcmul_(zn, proj, value=-1.0) / norm).reshape(n, num_pq * d)
         return g_rows, g_books, None, None, None
 

@@ -155,3 +155,34 @@ def test_largest_numbers_of_every_type(fmt, native, dev):
         for r, c in ((2, 0), (3, 0), (5, 1)):
             assert abs(float(finite[r, c] - x[r, c].to(F64))) <= step / 2 * 2.0 ** top, (dtype, r)
         assert bool((finite[:, 2:] == 0).all())                       # zeros beside them stay zeros: no NaN
+
+
+@pytest.mark.parametrize("branch", ["none", "closed form", "int8", "e4m3"])
+def test_quantiser_gradient_where_the_norm_is_clamped(branch, pkg, native, dev, monkeypatch):
+    """0 < |z| < 1e-12: the norm is the constant 1e-12 there and its derivative zero, so nothing is projected out, as autograd has
+    it through clamp_min in fp64.  A dozen roundings at most on the terms' magnitudes, 64 u where the norm is the row's own."""
+    monkeypatch.setattr(pkg.pqgo._PQStraightThrough, "hip_backward", branch != "closed form")
+    keep = branch if branch in ("int8", "e4m3") else "none"
+    torch.manual_seed(15)
+    n, p, k, d, beta, book = 120, 2, 32, 32, 0.25, 1.0
+    z = torch.randn(n, p, d) * torch.tensor([1.0, 1e-13, 3e-14, 1e-16])[torch.arange(n) % 4].reshape(n, 1, 1)
+    z = z.reshape(n, p * d).to(dev).requires_grad_(True)
+    books = (torch.randn(p, k, d, device=dev) * 0.2).requires_grad_(True)
+    g = torch.randn(n, p * d, device=dev)
+    zq, vq, idx = pkg.pqgo._PQStraightThrough.apply(z, books, beta, book, keep)
+    gz, gb = torch.autograd.grad([zq, vq], [z, books], [g, torch.tensor(300.0, device=dev)])
+    zk = z.detach() if keep == "none" else native.ckpt_unpack(native.ckpt_pack(z.detach(), keep))
+    z64, b64, i = zk.cpu().to(F64).requires_grad_(True), books.detach().cpu().to(F64).requires_grad_(True), idx.cpu()
+    z3 = z64.reshape(n, p, d)
+    norm = z3.norm(dim=-1, keepdim=True).clamp_min(1e-12)
+    zn, emb = z3 / norm, torch.stack([b64[q][i[q]] for q in range(p)], 1)
+    loss = 300.0 * (beta * ((zn - emb.detach()) ** 2).mean() + book * ((emb - zn.detach()) ** 2).mean()) + (zn.reshape(n, -1) * g.cpu().to(F64)).sum()
+    want_z, want_b = torch.autograd.grad(loss, [z64, b64])
+    s = 300.0 * 2 / (n * p * d)
+    size = (g.cpu().to(F64).reshape(n, p, d).norm(dim=-1, keepdim=True) + beta * s * (emb.norm(dim=-1, keepdim=True) + 1)) / norm
+    assert bool((norm[torch.arange(n) % 4 != 0] == 1e-12).all())
+    assert bool(((gz.cpu().to(F64) - want_z).abs().reshape(n, p, d) <= 64 * U * size).all())
+    terms = (book * s * (zn.abs() + emb.abs())).detach()
+    for q in range(p):
+        room, count = torch.zeros(k, d, dtype=F64).index_add_(0, i[q], terms[:, q]), torch.bincount(i[q], minlength=k).to(F64).unsqueeze(1)
+        assert bool(((gb[q].cpu().to(F64) - want_b[q]).abs() <= (count + 16) * U * room).all())
