@@ -4,7 +4,7 @@
 // The lookup writes its output once and reads the codebooks out of L2 (1 MB for 8 x 256 x 128 in fp32): it is bound by the
 // stores.  A lane owns 16 bytes of the output.  102400 rows, 8 x 256 x 128: bf16 39 us (5.3 TB/s of 211 MB), fp32 79 us (5.3 TB/s;
 // 86 with stores through the caches).  The gradient walks the rows in the order of their codes: code_sort.h.  Of the same rows in
-// fp32 it takes 97 us: 72 in the walk (5.9 TB/s of 419 MB), 18 in the sort, 6.5 in the join.
+// fp32 it takes 96 us: 72 in the walk (5.9 TB/s of 419 MB), 18 in the sort, 6.3 in the join.
 #include "code_sort.h"
 
 namespace {

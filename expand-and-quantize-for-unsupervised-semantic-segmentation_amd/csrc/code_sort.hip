@@ -53,7 +53,8 @@ __global__ __launch_bounds__(kCountThreads) void code_count_kernel(const Source 
 // one-pass sorts (whose bins are the codes), or null.  What this kernel waits for is latency: a wave's pairs are loaded eight
 // times 64 at once (and kept where that is all of them), the chunks' counts sixteen at once.  Many waves a workgroup make few
 // chunks, i.e. few counts to read for each: 102400 rows, 8 sub-spaces, both kernels: 15.8 us with 16 waves and 15 chunks, 18.3 us
-// with 4 waves and 50 chunks; two kernels that only launch and load take 9.
+// with 4 waves and 50 chunks; two kernels that only launch and load take 9.  (Called over and over; in a lookup's gradient, with
+// what else runs there in the caches, 17.7.)
 template <int WAVES, int BINS>                          // bins <= BINS, a multiple or a fraction of the threads
 __global__ __launch_bounds__(64 * WAVES) void code_place_kernel(const Source s, const uint32_t* __restrict__ table, CodePair* __restrict__ dst,
                                                                uint32_t* __restrict__ starts, int chunk_rows, int shift, int bits) {

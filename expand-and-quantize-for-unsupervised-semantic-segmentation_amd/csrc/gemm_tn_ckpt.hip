@@ -200,11 +200,11 @@ __global__ __launch_bounds__(kTnThreads, 2) void gemm_tn_ckpt_kernel(const Args 
 // without a branch in between, so that the scheduler can put all of it between the MFMAs.  The loop goes by four stages, so that
 // slots and register sets are constants.  Loads past a workgroup's rows return zero (buffer addressing), codes and scales too:
 // the last stages need no care and the surplus ones of the last round multiply zeros.
-// Conversions, address arithmetic and the bias are what the matrix pipe waits for (counted: of 75 M issue cycles of the first
-// version with one wave a SIMD, the MFMAs took 39 M and other vector instructions 23 M, one after the other); hence two waves
-// a SIMD, constant LDS addresses and buffer loads.
-// 102400 rows, 1024 x 768, bias and join included: int8 170 us, e4m3 (whose conversion is one instruction for two values) 159 us,
-// 0.95 and 1.01 PFLOP/s; an 8192^3 bf16 library product runs at 1.25.  Another 102400 rows add 130 and 128 us (1.24 and 1.26
+// Conversions, address arithmetic and the bias are what the matrix pipe waits for; hence two waves a SIMD, constant LDS addresses
+// and buffer loads.  Counted at 102400 rows, 1024 x 768, int8: 5.0 million MFMAs hold the matrix pipes for 54 % of the launch,
+// beside 22 million other vector instructions; 327 MB read, 69 written.
+// 102400 rows, 1024 x 768, bias and join included: int8 165 us, e4m3 (whose conversion is one instruction for two values) 160 us,
+// 0.98 and 1.01 PFLOP/s; an 8192^3 bf16 library product runs at 1.25.  Another 102400 rows add 130 and 128 us (1.24 and 1.26
 // PFLOP/s); what does not grow with the rows, the partial products (256 KB a CU) and their join among it, is 30 to 40 us.
 // Consecutive row ranges and tiles on one XCD: 175 us, 184 dealt round (102400 rows, 384 x 384: 55 / 70).  The large tile spills
 // a few registers, 24 bytes a lane; two of them are read back in each stage of the int8 form.

@@ -4,8 +4,9 @@
 // Rows are walked in the order of their codes, so a codeword is loaded once for a run of rows, the sum of (zn - emb) over the
 // run stays in registers, and every (row, sub-space) is still visited once: its part of g_zq is read and its part of g_z
 // written there.  A part is d consecutive elements (512 bytes of g_zq and g_z at d = 128): whole cache lines, so the order costs
-// no extra traffic.  102400 rows, 8 x 256 x 128, int8: 217 us with a gradient of z_q (955 MB at 4.8 TB/s in the walk, 24 us for the
-// sort and the join, each kernel timed by itself), 120 us without; bound by memory (a copy of 1 GiB: 5.15 TB/s).
+// little extra traffic.  102400 rows, 8 x 256 x 128, int8: the walk takes 195 us with a gradient of z_q (955 MB at 4.9 TB/s; counted,
+// 603 MB read and 427 written) and 102 without, as the training step has it; sort and join 24.  Bound by memory (a copy of 1 GiB:
+// 5.15 TB/s).
 //
 // With n = max(|z|, 1e-12), zn = z / n, s = g_vq 2 / (rows d num_pq), the gradient of zn is g_zq + beta s (zn - emb), and
 //     g_z = (g' - zn <zn, g'>) / n,   g' = g_zq - beta s emb
