@@ -176,8 +176,9 @@ __global__ __launch_bounds__(256) void code_accumulate_kernel(const Op op, const
 
 // WAVES = 4: a wave owns a code, and the chain of partial sums of a long run is shared by the workgroup's four waves.  WAVES = 16,
 // where there are few codes, i.e. long runs: a workgroup owns a code (102045 rows, 5 x 2 x 32, gradient of a lookup: 42 us, 65 us
-// with four waves; 102400 rows, 8 x 256 x 128: 100 / 96 us; hence at most 1024 workgroups, a codeword of more than 256 columns
-// taking several: 3000 rows, 1000 x 4096: 81 us with 16000 of them, 36 with four waves each).
+// with four waves; 102400 rows, 8 x 256 x 128: 100 / 96 us, hence at most 1024 codes), and at most 2048 workgroups, a codeword of
+// more than 256 columns taking several (3000 rows, 1000 x 4096, 16000 workgroups: 81 us, 36 with four waves each; 20000 rows of one
+// code, 600 x 512, 1200 workgroups: 55 / 74).
 template <int LPR, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void code_join_kernel(const WalkArgs w) {
     constexpr int SLOTS = 64 / LPR, CODES = WAVES == 4 ? 4 : 1, kLong = 16 * SLOTS, F = 8;
@@ -522,7 +523,7 @@ int walk_launch_lpr(const Op& op, const SortPlan& s, const IndexView& index, cha
     else hipLaunchKernelGGL((code_accumulate_kernel<Op, LPR, 2>), grid, dim3(256), 0, stream, op, w);
     rc = check_launch("code_accumulate_kernel");
     if (rc != EQUSS_OK || !out) return rc;
-    if ((int64_t)s.K * s.num_pq * cchunks <= 1024) hipLaunchKernelGGL((code_join_kernel<LPR, 16>), dim3(s.K, s.num_pq, cchunks), dim3(1024), 0, stream, w);
+    if ((int64_t)s.K * s.num_pq <= 1024 && (int64_t)s.K * s.num_pq * cchunks <= 2048) hipLaunchKernelGGL((code_join_kernel<LPR, 16>), dim3(s.K, s.num_pq, cchunks), dim3(1024), 0, stream, w);
     else
         for (constexpr int64_t kMost = max_blocks(256) * 4; w.code0 < (int64_t)s.K; w.code0 += kMost) {   // (one launch below 67 million codes)
             const int64_t left = (int64_t)s.K - w.code0, codes = left < kMost ? left : kMost;

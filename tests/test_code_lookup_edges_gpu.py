@@ -146,3 +146,16 @@ def test_lookup_of_the_widest_codewords(num_pq, d, dtype, native, dev):
         assert torch.equal(got[r], want), r
     g = torch.ones(5, num_pq * d, dtype=dtype, device=dev)
     assert torch.equal(native.code_lookup_grad(g, idx.to(dev), 3).cpu(), torch.ones(num_pq, 3, d))
+
+
+@pytest.mark.parametrize("rows,num_pq,k,d", [(3000, 1, 300, 2000), (2500, 1, 1000, 1100), (5000, 2, 40, 1500), (9000, 1, 2100, 515)])
+def test_lookup_gradient_of_wide_codewords_is_exact_on_whole_numbers(rows, num_pq, k, d, native, dev):
+    """Rows of several waves, on either side of the border between the joins of 16 and of four waves a code."""
+    g = torch.randint(-8, 9, (rows, num_pq * d), generator=torch.Generator().manual_seed(44)).float()
+    for kind in ("low", "busy", "padding"):
+        idx = clustered(kind, num_pq, rows, k, 45)
+        want = torch.zeros(num_pq, k, d)
+        for p in range(num_pq):
+            ok = idx[p] >= 0
+            want[p].index_add_(0, idx[p][ok], g.reshape(rows, num_pq, d)[ok, p])
+        assert torch.equal(native.code_lookup_grad(g.to(dev), idx.to(dev), k).cpu(), want), kind
